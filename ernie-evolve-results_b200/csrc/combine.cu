@@ -17,7 +17,12 @@
 // 16-byte peer loads over NVLink inside the same kernel that weights and adds
 // it: the return all-to-all and the un-permute are one pass, and no receive
 // buffer exists.  Arithmetic and order are those of the local form.
+//
+// moe_rd_unsort_tokens is the same kernel for rows of any element type, with the
+// weights left out on request (w = 1: the gradient of moe_rd_sort_tokens) and with
+// every row index checked against the number of rows of y.
 #include "common.cuh"
+#include "row_types.cuh"
 
 namespace moe_rd {
 namespace {
@@ -29,11 +34,12 @@ constexpr int kCombineBlocksPerSm = 64;
 struct CombineArgs {
   const uint4* y;
   const int32_t* inverse_perm;
-  const float* weights;
+  const float* weights;  // or null: every weight is 1
   const uint4* shared;
   uint4* out;
   int64_t T;
   int nvec, K;
+  uint32_t y_rows;       // row indices at or past this (and negative ones) are pairs without a row
   // EP: y of rank d is peer_y[d]; pair (t,k) of expert e is row
   // dest_base[e] + (inverse_perm[t,k] - offsets[e]) there
   const uint4* peer_y[8];
@@ -55,20 +61,27 @@ __device__ __forceinline__ const uint4* row_of(const CombineArgs& a, int64_t t, 
   return a.peer_y[e / a.epr] + (size_t)row * a.nvec;
 }
 
-__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
+template <bool EP>
+__device__ __forceinline__ int position_of(const CombineArgs& a, int64_t t, int k) {
+  if (k >= a.K) return -1;
+  const int pos = __ldg(a.inverse_perm + (size_t)t * a.K + k);
+  return !EP && (uint32_t)pos >= a.y_rows ? -1 : pos;
 }
 
-template <int KT, bool EP>
+__device__ __forceinline__ float weight_of(const CombineArgs& a, int64_t t, int k) {
+  if (k >= a.K) return 0.0f;
+  return a.weights != nullptr ? __ldg(a.weights + (size_t)t * a.K + k) : 1.0f;
+}
+
+template <int KT, bool EP, int DT>
 __device__ __forceinline__ void combine_unit(const CombineArgs& a, int64_t t, int v) {
   int pos[KT];
   float w[KT];
   uint4 yv[KT];
 #pragma unroll
   for (int k = 0; k < KT; ++k) {
-    pos[k] = k < a.K ? __ldg(a.inverse_perm + (size_t)t * a.K + k) : -1;
-    w[k] = k < a.K ? __ldg(a.weights + (size_t)t * a.K + k) : 0.0f;
+    pos[k] = position_of<EP>(a, t, k);
+    w[k] = weight_of(a, t, k);
   }
 #pragma unroll
   for (int k = 0; k < KT; ++k) {
@@ -80,41 +93,38 @@ __device__ __forceinline__ void combine_unit(const CombineArgs& a, int64_t t, in
         yv[k] = __ldcs(src + v);
     }
   }
-  float acc[8];
+  constexpr int NE = RowVec<DT>::N;
+  float acc[NE];
   if (a.shared != nullptr) {
     const uint4 s = __ldcs(a.shared + (size_t)t * a.nvec + v);
-    unpack8(s, acc);
+    RowVec<DT>::unpack(s, acc);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
+    for (int j = 0; j < NE; ++j) acc[j] = 0.0f;
   }
 #pragma unroll
   for (int k = 0; k < KT; ++k) {
     if (pos[k] >= 0) {
-      float f[8];
-      unpack8(yv[k], f);
+      float f[NE];
+      RowVec<DT>::unpack(yv[k], f);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] = fmaf(w[k], f[j], acc[j]);
+      for (int j = 0; j < NE; ++j) acc[j] = fmaf(w[k], f[j], acc[j]);
     }
   }
-  uint4 o;
-  o.x = pack_bf16x2(acc[0], acc[1]);
-  o.y = pack_bf16x2(acc[2], acc[3]);
-  o.z = pack_bf16x2(acc[4], acc[5]);
-  o.w = pack_bf16x2(acc[6], acc[7]);
-  __stcs(a.out + (size_t)t * a.nvec + v, o);
+  __stcs(a.out + (size_t)t * a.nvec + v, RowVec<DT>::pack(acc));
 }
 
 // K > 8: same arithmetic with the loads issued eight at a time.
-template <bool EP>
+template <bool EP, int DT>
 __device__ __forceinline__ void combine_unit_any(const CombineArgs& a, int64_t t, int v) {
-  float acc[8];
+  constexpr int NE = RowVec<DT>::N;
+  float acc[NE];
   if (a.shared != nullptr) {
     const uint4 s = __ldcs(a.shared + (size_t)t * a.nvec + v);
-    unpack8(s, acc);
+    RowVec<DT>::unpack(s, acc);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
+    for (int j = 0; j < NE; ++j) acc[j] = 0.0f;
   }
   for (int k0 = 0; k0 < a.K; k0 += 8) {
     int pos[8];
@@ -122,8 +132,8 @@ __device__ __forceinline__ void combine_unit_any(const CombineArgs& a, int64_t t
     uint4 yv[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      pos[k] = k0 + k < a.K ? __ldg(a.inverse_perm + (size_t)t * a.K + k0 + k) : -1;
-      w[k] = k0 + k < a.K ? __ldg(a.weights + (size_t)t * a.K + k0 + k) : 0.0f;
+      pos[k] = position_of<EP>(a, t, k0 + k);
+      w[k] = weight_of(a, t, k0 + k);
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -138,22 +148,17 @@ __device__ __forceinline__ void combine_unit_any(const CombineArgs& a, int64_t t
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       if (pos[k] >= 0) {
-        float f[8];
-        unpack8(yv[k], f);
+        float f[NE];
+        RowVec<DT>::unpack(yv[k], f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] = fmaf(w[k], f[j], acc[j]);
+        for (int j = 0; j < NE; ++j) acc[j] = fmaf(w[k], f[j], acc[j]);
       }
     }
   }
-  uint4 o;
-  o.x = pack_bf16x2(acc[0], acc[1]);
-  o.y = pack_bf16x2(acc[2], acc[3]);
-  o.z = pack_bf16x2(acc[4], acc[5]);
-  o.w = pack_bf16x2(acc[6], acc[7]);
-  __stcs(a.out + (size_t)t * a.nvec + v, o);
+  __stcs(a.out + (size_t)t * a.nvec + v, RowVec<DT>::pack(acc));
 }
 
-template <int KT, bool EP>
+template <int KT, bool EP, int DT>
 __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const CombineArgs a) {
   pdl_sync();
   const int lane = threadIdx.x & 31;
@@ -165,9 +170,9 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const CombineA
     const int v = (int)(u - t * upr) * 32 + lane;
     if (v >= a.nvec) continue;
     if (KT > 0)
-      combine_unit<(KT > 0 ? KT : 1), EP>(a, t, v);
+      combine_unit<(KT > 0 ? KT : 1), EP, DT>(a, t, v);
     else
-      combine_unit_any<EP>(a, t, v);
+      combine_unit_any<EP, DT>(a, t, v);
   }
 }
 
@@ -182,10 +187,10 @@ using namespace moe_rd;
 namespace moe_rd {
 namespace {
 
-template <bool EP>
+template <bool EP, int DT = MOE_RD_T_BF16>
 int launch_combine(CombineArgs& a, int64_t T, int32_t H, int32_t K, void* stream) {
   a.T = T;
-  a.nvec = H / 8;
+  a.nvec = H / RowVec<DT>::N;
   a.K = K;
   const int64_t units = T * ((a.nvec + 31) / 32);
   const int64_t want = (units + kCombineWarps - 1) / kCombineWarps;
@@ -194,14 +199,15 @@ int launch_combine(CombineArgs& a, int64_t T, int32_t H, int32_t K, void* stream
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (K <= 2)
-    e = launch_pdl(combine_kernel<2, EP>, grid, dim3(kCombineThreads), 0, s, a);
+    e = launch_pdl(combine_kernel<2, EP, DT>, grid, dim3(kCombineThreads), 0, s, a);
   else if (K <= 4)
-    e = launch_pdl(combine_kernel<4, EP>, grid, dim3(kCombineThreads), 0, s, a);
+    e = launch_pdl(combine_kernel<4, EP, DT>, grid, dim3(kCombineThreads), 0, s, a);
   else if (K <= 8)
-    e = launch_pdl(combine_kernel<8, EP>, grid, dim3(kCombineThreads), 0, s, a);
+    e = launch_pdl(combine_kernel<8, EP, DT>, grid, dim3(kCombineThreads), 0, s, a);
   else
-    e = launch_pdl(combine_kernel<0, EP>, grid, dim3(kCombineThreads), 0, s, a);
+    e = launch_pdl(combine_kernel<0, EP, DT>, grid, dim3(kCombineThreads), 0, s, a);
   count_launch();
+  if (e != cudaSuccess) set_last_cuda_error(e);
   return e == cudaSuccess ? MOE_RD_OK : MOE_RD_E_CUDA;
 }
 
@@ -308,7 +314,30 @@ extern "C" int moe_rd_combine(int64_t T, int32_t H, int32_t K, const void* y,
   a.weights = combine_weights;
   a.shared = static_cast<const uint4*>(shared);
   a.out = static_cast<uint4*>(out);
+  a.y_rows = 0x7fffffffu;
   return launch_combine<false>(a, T, H, K, stream);
+}
+
+extern "C" int moe_rd_unsort_tokens(int64_t T, int32_t H, int32_t K, int32_t dtype, const void* y, int64_t y_rows,
+                                    const int32_t* inverse_perm, const float* weights, const void* shared,
+                                    void* out, void* stream) {
+  const int rc = check_rows(T, H, K, dtype, y_rows);
+  if (rc != MOE_RD_OK) return rc;
+  if (T == 0) return MOE_RD_OK;
+  if ((y == nullptr && y_rows > 0) || inverse_perm == nullptr || out == nullptr) return MOE_RD_E_NULL;
+  if ((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out) |
+       reinterpret_cast<uintptr_t>(shared)) & 15)
+    return MOE_RD_E_ALIGN;
+  CombineArgs a = {};
+  a.y = static_cast<const uint4*>(y);
+  a.inverse_perm = inverse_perm;
+  a.weights = weights;
+  a.shared = static_cast<const uint4*>(shared);
+  a.out = static_cast<uint4*>(out);
+  a.y_rows = (uint32_t)y_rows;
+  if (dtype == MOE_RD_T_BF16) return launch_combine<false, MOE_RD_T_BF16>(a, T, H, K, stream);
+  if (dtype == MOE_RD_T_FP16) return launch_combine<false, MOE_RD_T_FP16>(a, T, H, K, stream);
+  return launch_combine<false, MOE_RD_T_F32>(a, T, H, K, stream);
 }
 
 extern "C" int moe_rd_ep_combine(int64_t T, int32_t H, int32_t K, int32_t E, int32_t world,

@@ -98,7 +98,10 @@ static_assert(kMaxE <= kPosThreads, "tile mode keeps one expert per thread");
 // block-wide scan over the experts, offsets[e] = rows kept by the experts
 // before e (the scan part of offsets_kernel of the reference, kernel.cu:2074-2086).
 // Block 0 writes offsets[E+1] and the per-expert counts out.
-template <bool TILE>
+// SORT (moe_rd_sort_tokens; implies TILE): the ids come from the caller.  An id
+// outside [0, E) is a pair without an expert: it gets inverse_perm = -1 and is not
+// an error; the rows behind the last one get row_token = -1.
+template <bool TILE, bool SORT = false>
 __global__ void __launch_bounds__(kPosThreads) positions_kernel(const PositionArgs a) {
   extern __shared__ __align__(16) uint16_t s_cc[];  // [chunks][E]
   __shared__ int s_off[TILE ? kMaxE : 1], s_tb[TILE ? kMaxE : 1], s_tot[TILE ? kMaxE : 1], s_w[kPosThreads / 32];
@@ -187,6 +190,10 @@ __global__ void __launch_bounds__(kPosThreads) positions_kernel(const PositionAr
       }
     }
     if (tile == 0 && tid == 0) a.offsets[a.E] = all;
+    if (SORT) {
+      for (int64_t r = (int64_t)all + (int64_t)tile * kPosThreads + tid; r < a.out_rows; r += (int64_t)a.ntiles * kPosThreads)
+        a.row_token[r] = -1;
+    }
   }
   __syncthreads();
   for (int c = warp, k = 0; c < nch; c += nwarps, ++k) {
@@ -243,15 +250,15 @@ __global__ void __launch_bounds__(kPosThreads) positions_kernel(const PositionAr
     int pos = -1;
     bool dropped = false;
     if (e < 0) {
-      report(a.status, 1, e_raw, (int)s);
+      if (!SORT) report(a.status, 1, e_raw, (int)s);
     } else {
       const int64_t r = (int64_t)tb + s_cc[c * a.E + e] + __popc(m & ((1u << lane) - 1u));
       dropped = a.capacity > 0 && r >= a.capacity;
       if (!dropped) {
         const int64_t q = (int64_t)off + r;
-        if (q < 0 || q >= a.out_rows)
-          report(a.status, 2, (int)q, (int)s);
-        else
+        if (q < 0 || q >= a.out_rows) {
+          if (!SORT) report(a.status, 2, (int)q, (int)s);
+        } else
           pos = (int)q;
       }
     }
@@ -297,6 +304,8 @@ struct ScatterArgs {
   float* peer_scales[kMaxWorld];
   int epr;
   const int32_t* dense;  // identity experts whose rows are not written (or null)
+  int64_t out_rows;      // CLEAR_TAIL: rows [offsets[E], out_rows) are set to zero
+  int E;
 };
 
 // Destination of pair (t,k): local row index, or (peer buffer, row) when EP.
@@ -367,7 +376,7 @@ struct UnitWalk {
   }
 };
 
-template <int FMT, bool EP>
+template <int FMT, bool EP, bool CLEAR_TAIL = false>
 __global__ void __launch_bounds__(kScatterThreads) scatter_kernel(const ScatterArgs a) {
   pdl_trigger();
   const int lane = threadIdx.x & 31;
@@ -429,6 +438,17 @@ __global__ void __launch_bounds__(kScatterThreads) scatter_kernel(const ScatterA
           for (int u = 0; u < kUV; ++u)
             if (vb + 32 * u < nvec) store_row16(d + vb + 32 * u, val[u]);
         }
+      }
+    }
+    if (CLEAR_TAIL) {
+      const int64_t first = __ldg(a.offsets + a.E);
+      UnitWalk tw(w0, W, upr);
+      for (; first + tw.t < a.out_rows; tw.next()) {
+        uint4* d = reinterpret_cast<uint4*>(a.rows) + (size_t)(first + tw.t) * nvec;
+        const int vb = tw.c * (32 * kUV) + lane;
+#pragma unroll
+        for (int u = 0; u < kUV; ++u)
+          if (vb + 32 * u < nvec) store_row16(d + vb + 32 * u, make_uint4(0u, 0u, 0u, 0u));
       }
     }
   } else {
@@ -648,6 +668,49 @@ cudaError_t launch_scatter(const moe_rd_params& p, const moe_rd_buffers& b, cons
     e = launch_pdl(scatter_kernel<MOE_RD_ROWS_FP8_E4M3_B128, false>, dim3(grid), dim3(kScatterThreads), 0, s, a);
   else
     e = launch_pdl(scatter_kernel<MOE_RD_ROWS_BF16, false>, dim3(grid), dim3(kScatterThreads), 0, s, a);
+  count_launch();
+  return e;
+}
+
+// Positions and row copy of moe_rd_sort_tokens, from the counts that sort_count_kernel left.  A row copy does not
+// look at its elements: `H16` is the row length in units of 16 bits, whatever the type.
+cudaError_t launch_sort_scatter(int64_t T, int H16, int E, int K, int64_t capacity, int64_t out_rows, const void* x,
+                                const int32_t* ids, const int32_t* tile_counts, const int32_t* group_counts,
+                                void* rows, int32_t* offsets, int32_t* inverse_perm, int32_t* row_token,
+                                int32_t* counts, cudaStream_t s) {
+  PositionArgs pa = {};
+  pa.ids = ids;
+  pa.tile_base = tile_counts;
+  pa.group_counts = group_counts;
+  pa.offsets = offsets;
+  pa.inverse_perm = inverse_perm;
+  pa.row_token = row_token;
+  pa.user_counts = counts;
+  pa.T = T;
+  pa.capacity = capacity;
+  pa.out_rows = out_rows;
+  pa.E = E;
+  pa.K = K;
+  pa.ntiles = (int)((T + kTile - 1) / kTile);
+  cudaError_t e = launch_pdl(positions_kernel<true, true>, dim3((unsigned)pa.ntiles), dim3(kPosThreads),
+                             positions_smem(K, E), s, pa);
+  count_launch();
+  if (e != cudaSuccess) return e;
+  ScatterArgs a = {};
+  a.x = static_cast<const uint16_t*>(x);
+  a.inverse_perm = inverse_perm;
+  a.offsets = offsets;
+  a.rows = rows;
+  a.T = T;
+  a.H = H16;
+  a.K = K;
+  a.E = E;
+  a.out_rows = out_rows;
+  const int64_t units = T * (((H16 >> 3) + 32 * kUV - 1) / (32 * kUV));
+  const int64_t want = (units + kScatterWarps - 1) / kScatterWarps;
+  const int64_t cap = (int64_t)device_sms() * MOE_RD_SC_BLOCKS_PER_SM;
+  e = launch_pdl(scatter_kernel<MOE_RD_ROWS_BF16, false, true>, dim3((unsigned)(want < cap ? want : cap)),
+                 dim3(kScatterThreads), 0, s, a);
   count_launch();
   return e;
 }

@@ -1,0 +1,184 @@
+// Gradients of the weighted way back (moe_rd_unsort_tokens_backward):
+//   grad_y[pos(t,k),:] = w[t,k] * grad_out[t,:],    grad_w[t,k] = <grad_out[t,:], y[pos(t,k),:]>
+//
+// Walked token by token, so that grad_out is read once (row by row of y it would be read K times) while the rows of y
+// are gathered and the rows of grad_y scattered, each once, whole: HBM bounds it.  1 to 8 warps of a block share a
+// token, by the length of its row; a lane keeps one fp32 sum per slot over its vectors, in ascending order, the lanes
+// are added by a fixed tree and the warps in ascending order, so grad_w does not depend on scheduling.
+// Rows from *n_rows on belong to no pair: they are set to zero at the end, by all blocks.
+#include "row_types.cuh"
+
+namespace moe_rd {
+
+int device_sms();
+
+namespace {
+
+constexpr int kGradThreads = 256;
+constexpr int kGradWarps = kGradThreads / 32;
+constexpr int kGradBlocksPerSm = 16;
+
+struct UnsortGradArgs {
+  const uint4* grad_out;
+  const uint4* y;
+  const int32_t* inverse_perm;
+  const float* weights;   // or null: every weight is 1
+  const int32_t* n_rows;  // device value, or null: grad_y was cleared before
+  uint4* grad_y;          // or null
+  float* grad_weights;
+  int64_t T, y_rows;
+  int nvec, K;
+  int warps_per_token;    // 1, 2, 4 or 8
+};
+
+// KT slots at a time; NEED_W: grad_weights is wanted (and y is read).
+template <int DT, int KT, bool NEED_W>
+__global__ void __launch_bounds__(kGradThreads) unsort_grad_kernel(const UnsortGradArgs a) {
+  constexpr int NE = RowVec<DT>::N;
+  __shared__ float s_part[kGradWarps][KT];
+  pdl_sync();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int wpt = a.warps_per_token;
+  const int sub = warp & (wpt - 1);            // this warp's share of the token
+  const int tokens = kGradWarps / wpt;         // tokens of a block at a time
+  // every warp of the block makes the same number of trips: the barriers below are for all of them
+  for (int64_t base = (int64_t)blockIdx.x * tokens; base < a.T; base += (int64_t)gridDim.x * tokens) {
+    const int64_t t = base + warp / wpt;
+    const bool live = t < a.T;
+    for (int k0 = 0; k0 < a.K; k0 += KT) {
+      int pos[KT];
+      float w[KT], acc[KT];
+#pragma unroll
+      for (int k = 0; k < KT; ++k) {
+        pos[k] = live && k0 + k < a.K ? __ldg(a.inverse_perm + (size_t)t * a.K + k0 + k) : -1;
+        w[k] = live && k0 + k < a.K && a.weights != nullptr ? __ldg(a.weights + (size_t)t * a.K + k0 + k) : 1.0f;
+        acc[k] = 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+        if ((uint64_t)(int64_t)pos[k] >= (uint64_t)a.y_rows) pos[k] = -1;
+      if (live) {
+        for (int v = sub * 32 + lane; v < a.nvec; v += wpt * 32) {
+          const uint4 gv = __ldg(a.grad_out + (size_t)t * a.nvec + v);
+          uint4 yv[KT];
+          if (NEED_W) {
+#pragma unroll
+            for (int k = 0; k < KT; ++k)
+              if (pos[k] >= 0) yv[k] = __ldcs(a.y + (size_t)pos[k] * a.nvec + v);
+          }
+          float g[NE];
+          RowVec<DT>::unpack(gv, g);
+#pragma unroll
+          for (int k = 0; k < KT; ++k) {
+            if (pos[k] >= 0) {
+              if (NEED_W) {
+                float f[NE];
+                RowVec<DT>::unpack(yv[k], f);
+#pragma unroll
+                for (int j = 0; j < NE; ++j) acc[k] = fmaf(g[j], f[j], acc[k]);
+              }
+              if (a.grad_y != nullptr) {
+                float o[NE];
+#pragma unroll
+                for (int j = 0; j < NE; ++j) o[j] = __fmul_rn(w[k], g[j]);
+                __stcs(a.grad_y + (size_t)pos[k] * a.nvec + v, RowVec<DT>::pack(o));
+              }
+            }
+          }
+        }
+      }
+      if (NEED_W) {
+#pragma unroll
+        for (int k = 0; k < KT; ++k) acc[k] = warp_tree_sum(acc[k]);
+        if (lane == 0) {
+#pragma unroll
+          for (int k = 0; k < KT; ++k) s_part[warp][k] = acc[k];
+        }
+        __syncthreads();
+        if (live && sub == 0 && lane < KT && k0 + lane < a.K) {
+          float sum = s_part[warp][lane];
+          for (int i = 1; i < wpt; ++i) sum = __fadd_rn(sum, s_part[warp + i][lane]);
+          a.grad_weights[(size_t)t * a.K + k0 + lane] = sum;
+        }
+        __syncthreads();
+      }
+    }
+  }
+  if (a.grad_y != nullptr && a.n_rows != nullptr) {
+    int64_t n = __ldg(a.n_rows);
+    n = n < 0 ? 0 : n;
+    const int upr = (a.nvec + 31) >> 5;
+    for (int64_t u = (int64_t)blockIdx.x * kGradWarps + warp; u < (a.y_rows - n) * upr; u += (int64_t)gridDim.x * kGradWarps) {
+      const int64_t r = u / upr;
+      const int v = (int)(u - r * upr) * 32 + lane;
+      if (v < a.nvec) __stcs(a.grad_y + (size_t)(n + r) * a.nvec + v, make_uint4(0u, 0u, 0u, 0u));
+    }
+  }
+}
+
+template <int DT, bool NEED_W>
+cudaError_t launch_typed(const UnsortGradArgs& a, dim3 grid, cudaStream_t s) {
+  if (a.K <= 2) return launch_pdl(unsort_grad_kernel<DT, 2, NEED_W>, grid, dim3(kGradThreads), 0, s, a);
+  if (a.K <= 4) return launch_pdl(unsort_grad_kernel<DT, 4, NEED_W>, grid, dim3(kGradThreads), 0, s, a);
+  return launch_pdl(unsort_grad_kernel<DT, 8, NEED_W>, grid, dim3(kGradThreads), 0, s, a);
+}
+
+template <int DT>
+cudaError_t launch_dtype(const UnsortGradArgs& a, dim3 grid, cudaStream_t s) {
+  return a.grad_weights != nullptr ? launch_typed<DT, true>(a, grid, s) : launch_typed<DT, false>(a, grid, s);
+}
+
+}  // namespace
+}  // namespace moe_rd
+
+using namespace moe_rd;
+
+extern "C" int moe_rd_unsort_tokens_backward(int64_t T, int32_t H, int32_t K, int32_t dtype, const void* grad_out,
+                                             const void* y, int64_t y_rows, const int32_t* inverse_perm,
+                                             const float* weights, const int32_t* n_rows, void* grad_y,
+                                             float* grad_weights, void* stream) {
+  const int rc = check_rows(T, H, K, dtype, y_rows);
+  if (rc != MOE_RD_OK) return rc;
+  if (grad_y == nullptr && grad_weights == nullptr) return MOE_RD_E_NULL;
+  if (T > 0 && (grad_out == nullptr || inverse_perm == nullptr ||
+                (grad_weights != nullptr && y == nullptr && y_rows > 0)))
+    return MOE_RD_E_NULL;
+  if ((reinterpret_cast<uintptr_t>(grad_out) | reinterpret_cast<uintptr_t>(y) |
+       reinterpret_cast<uintptr_t>(grad_y)) & 15)
+    return MOE_RD_E_ALIGN;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
+  if (grad_y != nullptr && y_rows > 0 && (n_rows == nullptr || T == 0))
+    e = cudaMemsetAsync(grad_y, 0, (size_t)y_rows * H * (dtype == MOE_RD_T_F32 ? 4 : 2), s);
+  if (e == cudaSuccess && T > 0) {
+    UnsortGradArgs a = {};
+    a.grad_out = static_cast<const uint4*>(grad_out);
+    a.y = static_cast<const uint4*>(y);
+    a.inverse_perm = inverse_perm;
+    a.weights = weights;
+    a.n_rows = n_rows;
+    a.grad_y = y_rows > 0 ? static_cast<uint4*>(grad_y) : nullptr;
+    a.grad_weights = grad_weights;
+    a.T = T;
+    a.y_rows = y_rows;
+    a.nvec = dtype == MOE_RD_T_F32 ? H / 4 : H / 8;
+    a.K = K;
+    a.warps_per_token = a.nvec > 128 ? 8 : a.nvec > 64 ? 4 : a.nvec > 32 ? 2 : 1;
+    const int tokens = kGradWarps / a.warps_per_token;
+    const int64_t want = (T + tokens - 1) / tokens;
+    const int64_t cap = (int64_t)device_sms() * kGradBlocksPerSm;
+    const dim3 grid((unsigned)(want < cap ? want : cap));
+    if (dtype == MOE_RD_T_BF16)
+      e = launch_dtype<MOE_RD_T_BF16>(a, grid, s);
+    else if (dtype == MOE_RD_T_FP16)
+      e = launch_dtype<MOE_RD_T_FP16>(a, grid, s);
+    else
+      e = launch_dtype<MOE_RD_T_F32>(a, grid, s);
+    count_launch();
+  }
+  if (e != cudaSuccess) {
+    set_last_cuda_error(e);
+    return MOE_RD_E_CUDA;
+  }
+  return MOE_RD_OK;
+}

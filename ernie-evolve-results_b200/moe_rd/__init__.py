@@ -20,9 +20,13 @@ import torch
 
 from . import _cabi
 from ._cabi import MoeRdError  # noqa: F401
+from .experts import W4Weights, expert_matvec_w4, pack_w4  # noqa: F401
+from .sorting import (SortedTokens, UnsortGradients, routing_weights, routing_weights_backward, sort_tokens,  # noqa: F401
+                      unsort_tokens, unsort_tokens_backward)
 
 __all__ = ["route_dispatch", "combine", "combine_add_rows", "gemm_plan", "expert_stats", "RouteDispatchResult", "ExpertStats",
-           "MoeRdError", "capacity_from_factor"]
+           "MoeRdError", "capacity_from_factor", "sort_tokens", "unsort_tokens", "unsort_tokens_backward", "routing_weights",
+           "routing_weights_backward", "pack_w4", "expert_matvec_w4", "SortedTokens", "UnsortGradients", "W4Weights"]
 
 
 class RouteDispatchResult(NamedTuple):
@@ -52,9 +56,6 @@ def capacity_from_factor(factor: float, T: int, K: int, E: int) -> int:
 
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
-
-
-_BIAS_MODES = ("none", "logit", "select", "select_and_weight")
 
 
 def _impl(x, gate_weight, logit_bias, select_bias, given_logits, top_k, score_fn, n_groups,
@@ -183,8 +184,8 @@ def route_dispatch(hidden_states: torch.Tensor, gate_weight: Optional[torch.Tens
     ``hidden_states`` - for ``gemm_plan`` to aim that expert at ``hidden_states``
     (the reference's identity shortcut, kernel.cu:2089-2108).
     """
-    if bias_mode not in _BIAS_MODES:
-        raise ValueError(f"bias_mode must be one of {_BIAS_MODES}")
+    if bias_mode not in _cabi.BIAS_MODES:
+        raise ValueError(f"bias_mode must be one of {_cabi.BIAS_MODES}")
     logit_bias = bias if (bias is not None and bias_mode == "logit") else None
     select_bias = bias if (bias is not None and bias_mode in ("select", "select_and_weight")) else None
     T = hidden_states.numel() // hidden_states.shape[-1]

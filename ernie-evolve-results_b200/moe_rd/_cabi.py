@@ -8,6 +8,8 @@ from __future__ import annotations
 import ctypes
 from pathlib import Path
 
+import torch
+
 _LIB_PATH = Path(__file__).resolve().parent / "libmoe_rd.so"
 
 SCORE_FN = {"softmax": 0, "sigmoid": 1}
@@ -16,12 +18,16 @@ W_LAYOUT = {"HE": 0, "EH": 1}
 ROWS_FORMAT = {"bf16": 0, "fp8": 1}
 GATE_IMPL = {"auto": 0, "simt": 1, "umma": 2, "external": 3, "gemv": 4, "umma_one_cta": 5}
 SCATTER_IMPL = {"auto": 0, "simt": 1, "bulk": 2, "none": 3}
+ROW_DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+BIAS_MODES = ("none", "logit", "select", "select_and_weight")
 
 EXPORTS = (
     "moe_rd_workspace_bytes", "moe_rd_route_dispatch", "moe_rd_route_dispatch_noalloc",
     "moe_rd_route_dispatch_timed", "moe_rd_read_status", "moe_rd_ep_unpack", "moe_rd_ep_plan", "moe_rd_combine",
     "moe_rd_combine_add_rows",
     "moe_rd_ep_scatter", "moe_rd_ep_scatter_once", "moe_rd_ep_replicate", "moe_rd_ep_combine", "moe_rd_read_status_noalloc", "moe_rd_gemm_plan", "moe_rd_expert_stats",
+    "moe_rd_sort_workspace_bytes", "moe_rd_sort_tokens", "moe_rd_unsort_tokens", "moe_rd_unsort_tokens_backward",
+    "moe_rd_routing_weights", "moe_rd_routing_weights_backward", "moe_rd_expert_matvec_w4",
     "moe_rd_launch_count", "moe_rd_strerror", "moe_rd_last_cuda_error", "moe_rd_version",
 )
 
@@ -126,6 +132,17 @@ def lib() -> ctypes.CDLL:
         L.moe_rd_expert_stats.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p,
                                           ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
         L.moe_rd_expert_stats.restype = ctypes.c_int
+        ptr, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+        for name, argtypes in (
+                ("moe_rd_sort_workspace_bytes", [i64, i32, i32, ctypes.POINTER(ctypes.c_size_t)]),
+                ("moe_rd_sort_tokens", [i64, i32, i32, i32, i32, i64, i64] + [ptr] * 8 + [ctypes.c_size_t, ptr]),
+                ("moe_rd_unsort_tokens", [i64, i32, i32, i32, ptr, i64] + [ptr] * 5),
+                ("moe_rd_unsort_tokens_backward", [i64, i32, i32, i32, ptr, ptr, i64] + [ptr] * 6),
+                ("moe_rd_routing_weights", [i64, i32, i32, i32, i32, f32, f32] + [ptr] * 6),
+                ("moe_rd_routing_weights_backward", [i64, i32, i32, i32, i32, f32, f32] + [ptr] * 7),
+                ("moe_rd_expert_matvec_w4", [i64, i32, i32, i32, i32, i32] + [ptr] * 7)):
+            getattr(L, name).argtypes = argtypes
+            getattr(L, name).restype = ctypes.c_int
         L.moe_rd_read_status.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(ctypes.c_int32)]
         L.moe_rd_read_status.restype = ctypes.c_int
         L.moe_rd_launch_count.argtypes = []
@@ -157,3 +174,9 @@ def workspace_bytes(params: Params) -> int:
 
 def launch_count() -> int:
     return int(lib().moe_rd_launch_count())
+
+
+def sort_workspace_bytes(T: int, E: int, K: int) -> int:
+    n = ctypes.c_size_t(0)
+    check(lib().moe_rd_sort_workspace_bytes(T, E, K, ctypes.byref(n)))
+    return int(n.value)

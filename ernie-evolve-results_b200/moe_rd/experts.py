@@ -1,0 +1,117 @@
+"""Products of few rows with 4-bit expert weights: the expert layer of a decode step, between ``route_dispatch`` (or
+``sort_tokens``) and ``combine`` (or ``unsort_tokens``)."""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _cabi
+from ._cabi import ROW_DTYPE
+from .sorting import _aligned, _check_offsets, _ptr, call, check_device, check_out, wants_grad
+
+
+class W4Weights(NamedTuple):
+    """4-bit weights in the layout of the kernel (see ``moe_rd_expert_matvec_w4`` in include/moe_rd.h)."""
+    packed: torch.Tensor           # [E, ceil(N/16), ceil(K/128), 1024] uint8
+    scales: torch.Tensor           # [E, ceil(N/16), K/group, 16] bf16 or fp16
+    zeros: Optional[torch.Tensor]  # the same shape, uint8; None: every zero point is 8
+    N: int
+    K: int
+    group: int
+
+
+def _blocked(t: torch.Tensor) -> torch.Tensor:
+    """[E, N, G] per-group values as [E, ceil(N/16), G, 16], zero-padded."""
+    E, N, G = t.shape
+    full = t.new_zeros((E, -(-N // 16) * 16, G))
+    full[:, :N] = t
+    return full.reshape(E, -1, 16, G).transpose(2, 3).contiguous()
+
+
+def pack_w4(q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None) -> W4Weights:
+    """Lay 4-bit weights out for ``expert_matvec_w4``; done once, when a program loads them (on the CPU or a GPU).
+
+    q: [E, N, K/2] uint8 (or [N, K/2] for one matrix), byte b holding input 2b in its low and 2b+1 in its high four bits;
+    scales: [E, N, K/group] bf16 or fp16, the type of the rows that will be multiplied; zeros: uint8 of the same shape,
+    0..15, or None for 8.  The weight is (q - zero) * scale.  K must be a multiple of group, group of 32.
+    """
+    if q.dim() == 2:
+        q, scales, zeros = q[None], scales[None], None if zeros is None else zeros[None]
+    if q.dtype != torch.uint8 or q.dim() != 3:
+        raise TypeError("pack_w4: q must be a uint8 tensor [E, N, K/2]")
+    if scales.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("pack_w4: scales must be bfloat16 or float16")
+    E, N, half = q.shape
+    K = 2 * half
+    if scales.dim() != 3 or scales.shape[:2] != q.shape[:2] or scales.shape[2] < 1 or N < 1 or E < 1 or K < 32:
+        raise ValueError("pack_w4: scales must be [E, N, K/group]")
+    G = scales.shape[2]
+    group = K // G
+    if K % G or group % 32:
+        raise ValueError(f"pack_w4: {G} scales for {K} inputs: groups must be equal and multiples of 32")
+    if zeros is not None:
+        if zeros.dtype != torch.uint8 or zeros.shape != scales.shape:
+            raise ValueError("pack_w4: zeros must be a uint8 tensor like scales")
+        if zeros.numel() and int(zeros.max()) > 15:
+            raise ValueError("pack_w4: zero points must be 0..15")
+    for t in (scales, zeros):
+        if t is not None and t.device != q.device:
+            raise ValueError("pack_w4: all tensors must be on one device")
+    blocks, chunks = -(-N // 16), -(-K // 128)
+    full = q.new_zeros((E, blocks * 16, chunks * 64))
+    full[:, :N, :half] = q
+    # [E, block, half, output, chunk, word i, lane j, byte] -> [E, block, chunk, half, output, j, i, byte]
+    r = full.reshape(E, blocks, 2, 8, chunks, 4, 4, 4).permute(0, 1, 4, 2, 3, 6, 5, 7)
+    packed = torch.empty(r.shape, dtype=torch.uint8, device=q.device)
+    packed[..., 0] = (r[..., 0] & 15) | ((r[..., 1] & 15) << 4)
+    packed[..., 1] = (r[..., 2] & 15) | ((r[..., 3] & 15) << 4)
+    packed[..., 2] = (r[..., 0] >> 4) | (r[..., 1] & 0xF0)
+    packed[..., 3] = (r[..., 2] >> 4) | (r[..., 3] & 0xF0)
+    return W4Weights(packed.reshape(E, blocks, chunks, 1024), _blocked(scales), None if zeros is None else _blocked(zeros), N, K, group)
+
+
+def expert_matvec_w4(x: torch.Tensor, weights: W4Weights, offsets: Optional[torch.Tensor] = None, *,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[r] = W_e x[r] for the rows r of every expert e, with 4-bit weights; [R, N] of the type of x.
+
+    x: [R, K] bf16 or fp16 rows in expert order (``permuted`` / ``rows``), of the type of the scales; offsets: [E+1] int32
+    device tensor as ``route_dispatch`` and ``sort_tokens`` return it, or None for one matrix that every row goes
+    through.  Rows that no expert has become zero.  Products are added in fp32 and rounded once.
+
+    Meant for few rows per expert (the weights are read once per eight rows of an expert); right for any number.  For
+    inference: a row that requires a gradient is refused.
+    """
+    if not isinstance(weights, W4Weights):
+        raise TypeError("expert_matvec_w4: weights must come from pack_w4")
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("expert_matvec_w4: rows must be bfloat16 or float16")
+    if weights.scales.dtype != x.dtype:
+        raise TypeError("expert_matvec_w4: rows and scales must have one type")
+    N, K = weights.N, weights.K
+    E, blocks, chunks = weights.packed.shape[:3]
+    G = K // weights.group
+    if x.dim() != 2 or x.shape[1] != K:
+        raise ValueError(f"expert_matvec_w4: rows must be [R, {K}]")
+    if (weights.packed.shape != (E, -(-N // 16), -(-K // 128), 1024) or weights.packed.dtype != torch.uint8
+            or weights.scales.shape != (E, blocks, G, 16) or not weights.packed.is_contiguous() or not weights.scales.is_contiguous()
+            or (weights.zeros is not None and (weights.zeros.shape != weights.scales.shape or weights.zeros.dtype != torch.uint8
+                                               or not weights.zeros.is_contiguous()))):
+        raise ValueError("expert_matvec_w4: weights are not as pack_w4 returns them")
+    _check_offsets("expert_matvec_w4", offsets)
+    if offsets is None and E != 1:
+        raise ValueError("expert_matvec_w4: offsets are needed where there is more than one expert")
+    if offsets is not None and offsets.numel() != E + 1:
+        raise ValueError(f"expert_matvec_w4: offsets must have {E + 1} elements")
+    if wants_grad(x, weights.scales):
+        raise RuntimeError("expert_matvec_w4 is for inference and has no gradient: pass detached rows")
+    dev = check_device("expert_matvec_w4", x, weights.packed, weights.scales, weights.zeros, offsets)
+    x2 = _aligned(x)
+    R = x.shape[0]
+    if out is None:
+        out = torch.empty((R, N), dtype=x.dtype, device=dev)
+    else:
+        check_out("expert_matvec_w4", out, (R, N), x.dtype, dev, x2)
+    call(dev, _cabi.lib().moe_rd_expert_matvec_w4, R, N, K, E, weights.group, ROW_DTYPE[x.dtype], _ptr(x2), _ptr(weights.packed),
+         _ptr(weights.scales), _ptr(weights.zeros), _ptr(offsets), _ptr(out))
+    return out

@@ -1,0 +1,402 @@
+"""Tokens sorted by expert and back, and the routing weights, each with its gradient.
+
+``route_dispatch`` routes and dispatches in one call and is not differentiable.  The functions here are its parts for
+training and for routings that come from elsewhere: ``sort_tokens`` (rows in expert order for given expert ids),
+``unsort_tokens`` (the weighted way back) and ``routing_weights`` (the combine weights of chosen experts as a function
+of the logits).  Where an argument requires a gradient, autograd reaches the hand-written backward kernels; the same
+kernels are there as plain functions (``unsort_tokens_backward``, ``routing_weights_backward``; the gradient of the sort
+is ``unsort_tokens`` without weights), which are what a CUDA graph may record.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from . import _cabi
+from ._cabi import BIAS_MODES, ROW_DTYPE, SCORE_FN
+
+
+class SortedTokens(NamedTuple):
+    rows: torch.Tensor          # [R, H] the tokens' rows, experts ascending; zeros behind offsets[E]
+    offsets: torch.Tensor       # [E+1] int32, offsets[E] = rows in use
+    inverse_perm: torch.Tensor  # [T, K] int32 row of every pair, -1 = none
+    row_token: torch.Tensor     # [R] int32 token of every row, -1 behind offsets[E]
+    counts: torch.Tensor        # [E] int32 pairs per expert before dropping
+
+
+class UnsortGradients(NamedTuple):
+    rows: Optional[torch.Tensor]     # [R, H] gradient of the expert outputs
+    weights: Optional[torch.Tensor]  # [T, K] fp32 gradient of the weights
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def check_device(name: str, *tensors: Optional[torch.Tensor]) -> torch.device:
+    """The one CUDA device of all the tensors."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name}: all tensors must be on one device, got {dev} and {t.device}")
+    if dev.type != "cuda":
+        raise RuntimeError(f"moe_rd.{name} has no CPU path: its tensors must be CUDA tensors")
+    return dev
+
+
+def call(dev: torch.device, entry, *args) -> None:
+    """Enqueue a C entry point on the current stream of ``dev``."""
+    if dev.index == torch.cuda.current_device():
+        _cabi.check(entry(*args, torch.cuda.current_stream(dev).cuda_stream))
+    else:
+        with torch.cuda.device(dev):
+            _cabi.check(entry(*args, torch.cuda.current_stream(dev).cuda_stream))
+
+
+def check_out(name: str, out: torch.Tensor, shape, dtype, dev: torch.device, *inputs: Optional[torch.Tensor]) -> torch.Tensor:
+    """``out`` is a buffer the call may write: of this shape and type, contiguous, apart from the inputs."""
+    if out.shape != torch.Size(shape) or out.dtype != dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"{name}: out must be a contiguous {dtype} tensor of shape {tuple(shape)} on {dev}")
+    if out.requires_grad:
+        raise ValueError(f"{name}: out must not require a gradient")
+    lo = out.data_ptr()
+    hi = lo + out.numel() * out.element_size()
+    for t in inputs:
+        if t is not None and lo < hi and t.numel() and t.data_ptr() < hi and lo < t.data_ptr() + t.numel() * t.element_size():
+            raise ValueError(f"{name}: out must not share memory with an input")
+    return out
+
+
+def wants_grad(*tensors: Optional[torch.Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _not_while_capturing(name: str, instead: str) -> None:
+    # A captured backward pass can end the process when an eager graph of the same leaves is alive, and nothing
+    # here can see whether one is; the plain functions do not go through the autograd engine.
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"moe_rd.{name}: autograd is not recorded into a CUDA graph; capture {instead} instead")
+
+
+def _check_ids(name: str, ids: torch.Tensor) -> Tuple[int, int]:
+    if ids.dtype != torch.int32:
+        raise TypeError(f"{name}: row and expert indices must be int32")
+    if ids.dim() != 2 or ids.shape[1] < 1:
+        raise ValueError(f"{name}: row and expert indices must be [T, K]")
+    return ids.shape[0], ids.shape[1]
+
+
+def _check_rows(name: str, rows: torch.Tensor) -> int:
+    if rows.dtype not in ROW_DTYPE:
+        raise TypeError(f"{name}: rows must be bfloat16, float16 or float32")
+    if rows.dim() < 2 or rows.shape[-1] < 1 or rows.shape[-1] * rows.element_size() % 16:
+        raise ValueError(f"{name}: rows must be [..., H] with H * element size a multiple of 16 bytes")
+    return rows.shape[-1]
+
+
+def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """Dense and 16-byte aligned (a view may start anywhere)."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+# --- sort ------------------------------------------------------------------------------------------------------------
+def _sort(x, expert_ids, num_experts, capacity, out):
+    H = x.shape[-1]
+    T, K = expert_ids.shape
+    E = num_experts
+    dev = x.device
+    x2 = _aligned(x.reshape(T, H))
+    ids = expert_ids.contiguous()
+    R = min(T * K, E * capacity) if capacity else T * K
+    if out is None:
+        new = lambda *shape, dtype=torch.int32: torch.empty(shape, dtype=dtype, device=dev)  # noqa: E731
+        out = SortedTokens(new(R, H, dtype=x.dtype), new(E + 1), new(T, K), new(R), new(E))
+    else:
+        check_out("sort_tokens", out.rows, (R, H), x.dtype, dev, x2, ids)
+        for t, shape in ((out.offsets, (E + 1,)), (out.inverse_perm, (T, K)), (out.row_token, (R,)), (out.counts, (E,))):
+            check_out("sort_tokens", t, shape, torch.int32, dev, ids)
+        if out.rows.data_ptr() % 16:
+            raise ValueError("sort_tokens: out.rows must be 16-byte aligned")
+    ws_bytes = _cabi.sort_workspace_bytes(T, E, K)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    call(dev, _cabi.lib().moe_rd_sort_tokens, T, H, E, K, ROW_DTYPE[x.dtype], capacity, R, _ptr(x2), _ptr(ids), _ptr(out.rows),
+         _ptr(out.offsets), _ptr(out.inverse_perm), _ptr(out.row_token), _ptr(out.counts), _ptr(ws), ws_bytes)
+    return out
+
+
+class _SortTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, expert_ids, num_experts, capacity):
+        out = _sort(x, expert_ids, num_experts, capacity, None)
+        ctx.save_for_backward(out.inverse_perm)
+        ctx.shape = x.shape
+        ctx.mark_non_differentiable(*out[1:])
+        return tuple(out)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_rows, *_):
+        _not_while_capturing("sort_tokens", "sort_tokens on detached tensors and unsort_tokens for its gradient")
+        (inverse_perm,) = ctx.saved_tensors
+        return _unsort(grad_rows, inverse_perm, None, None, None).reshape(ctx.shape), None, None, None
+
+
+def sort_tokens(x: torch.Tensor, expert_ids: torch.Tensor, num_experts: int, *, capacity: int = 0,
+                out: Optional[SortedTokens] = None) -> SortedTokens:
+    """Rows of ``x`` in expert order: ``rows[inverse_perm[t, k]] = x[t]`` for every pair (t, k) that has a row.
+
+    x: [..., H] bf16, fp16 or fp32 (any strides; H * element size a multiple of 16 bytes), T tokens in all.
+    expert_ids: [T, K] int32; an id outside [0, num_experts) is a pair without an expert (a padded token has K of
+    them), and one expert may occur twice for a token.  ``capacity`` keeps that many rows per expert, in (token, slot)
+    order, as in ``route_dispatch``; 0 keeps all.  The order inside an expert is the stable (token, slot) order.
+    Rows behind ``offsets[-1]`` are zero, with ``row_token`` -1.  At most 256 experts and 32 ids per token.
+
+    Differentiable in ``x``; the gradient is ``unsort_tokens(grad_rows, inverse_perm)``.  ``out`` takes the result of
+    an earlier call of the same sizes and reuses its buffers (not where ``x`` requires a gradient).
+    """
+    H = _check_rows("sort_tokens", x)
+    T, K = _check_ids("sort_tokens", expert_ids)
+    if x.numel() != T * H:
+        raise ValueError(f"sort_tokens: {x.numel() // H} tokens, but expert ids for {T}")
+    if num_experts < 1 or capacity < 0:
+        raise ValueError("sort_tokens: num_experts must be positive and capacity not negative")
+    num_experts, capacity = int(num_experts), int(capacity)
+    check_device("sort_tokens", x, expert_ids)
+    if not wants_grad(x):
+        return _sort(x, expert_ids, num_experts, capacity, out)
+    if out is not None:
+        raise ValueError("sort_tokens: out cannot be given where x requires a gradient")
+    _not_while_capturing("sort_tokens", "sort_tokens on detached tensors and unsort_tokens for its gradient")
+    return SortedTokens(*_SortTokens.apply(x, expert_ids, num_experts, capacity))
+
+
+# --- and back --------------------------------------------------------------------------------------------------------
+def _check_unsort(name, y, inverse_perm, weights, shared):
+    H = _check_rows(name, y)
+    T, K = _check_ids(name, inverse_perm)
+    if weights is not None:
+        if weights.dtype != torch.float32:
+            raise TypeError(f"{name}: weights must be float32")
+        if weights.shape != inverse_perm.shape:
+            raise ValueError(f"{name}: weights must be [T, K] like inverse_perm")
+    if shared is not None:
+        if shared.dtype != y.dtype:
+            raise TypeError(f"{name}: the [T, H] tensor must have the type of the rows")
+        if shared.dim() < 1 or shared.shape[-1] != H or shared.numel() != T * H:
+            raise ValueError(f"{name}: expected a tensor of T = {T} rows of {H}")
+    return T, K, H
+
+
+def _unsort(y, inverse_perm, weights, shared, out):
+    H = y.shape[-1]
+    T, K = inverse_perm.shape
+    dev = y.device
+    y2 = _aligned(y.reshape(-1, H))
+    inv = inverse_perm.contiguous()
+    w = None if weights is None else weights.contiguous()
+    sh = None if shared is None else _aligned(shared.reshape(T, H))
+    if out is None:
+        out = torch.empty((T, H), dtype=y.dtype, device=dev)
+    else:
+        check_out("unsort_tokens", out, (T, H), y.dtype, dev, y2, inv, w, sh)
+        if out.data_ptr() % 16:
+            raise ValueError("unsort_tokens: out must be 16-byte aligned")
+    call(dev, _cabi.lib().moe_rd_unsort_tokens, T, H, K, ROW_DTYPE[y.dtype], _ptr(y2), y2.shape[0], _ptr(inv), _ptr(w),
+         _ptr(sh), _ptr(out))
+    return out
+
+
+class _UnsortTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, inverse_perm, weights, shared, offsets):
+        out = _unsort(y, inverse_perm, weights, shared, None)
+        need_w = weights is not None and ctx.needs_input_grad[2]
+        ctx.save_for_backward(y if need_w else None, inverse_perm, weights, offsets)
+        ctx.y_shape = y.shape
+        ctx.shared_shape = None if shared is None else shared.shape
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        _not_while_capturing("unsort_tokens", "unsort_tokens on detached tensors and unsort_tokens_backward")
+        y, inverse_perm, weights, offsets = ctx.saved_tensors
+        need_y, need_w = ctx.needs_input_grad[0], weights is not None and ctx.needs_input_grad[2]
+        grad_y = grad_w = grad_shared = None
+        if need_y or need_w:
+            grad_y, grad_w = _unsort_backward(grad_out, y, ctx.y_shape, inverse_perm, weights, offsets, need_y, need_w, None)
+        if ctx.needs_input_grad[3]:
+            grad_shared = grad_out.reshape(ctx.shared_shape)
+        return grad_y, None, grad_w, grad_shared, None
+
+
+def unsort_tokens(y: torch.Tensor, inverse_perm: torch.Tensor, weights: Optional[torch.Tensor] = None,
+                  shared: Optional[torch.Tensor] = None, *, offsets: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[t] = shared[t] + sum_k weights[t, k] * y[inverse_perm[t, k]], rounded once from fp32.
+
+    ``combine`` for rows of any type (bf16, fp16, fp32), with a gradient.  y: [..., H] rows in expert order;
+    inverse_perm: [T, K] int32 as ``sort_tokens`` or ``route_dispatch`` return it (each row at most once; an index
+    outside the rows of y is a pair that contributes nothing, whatever its weight); weights: [T, K] fp32, or None for 1;
+    shared: T rows like y's, or None.
+
+    Differentiable in ``y``, ``weights`` and ``shared``.  With ``offsets`` (of the same sort) the gradient of ``y`` is
+    written in one pass; without it it is cleared first.  ``out`` takes a [T, H] buffer (not where a gradient is
+    required).
+    """
+    T, K, H = _check_unsort("unsort_tokens", y, inverse_perm, weights, shared)
+    check_device("unsort_tokens", y, inverse_perm, weights, shared, offsets)
+    _check_offsets("unsort_tokens", offsets)
+    if not wants_grad(y, weights, shared):
+        return _unsort(y, inverse_perm, weights, shared, out)
+    if out is not None:
+        raise ValueError("unsort_tokens: out cannot be given where a gradient is required")
+    _not_while_capturing("unsort_tokens", "unsort_tokens on detached tensors and unsort_tokens_backward")
+    return _UnsortTokens.apply(y, inverse_perm, weights, shared, offsets)
+
+
+def _check_offsets(name, offsets):
+    if offsets is not None and (offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() < 1 or not offsets.is_contiguous()):
+        raise TypeError(f"{name}: offsets must be a contiguous [E+1] int32 tensor")
+
+
+def _unsort_backward(grad_out, y, y_shape, inverse_perm, weights, offsets, need_y, need_w, out):
+    T, K = inverse_perm.shape
+    H = y_shape[-1]
+    R = 1
+    for n in y_shape[:-1]:
+        R *= n
+    dev = grad_out.device
+    g = _aligned(grad_out.reshape(T, H))
+    y2 = _aligned(y.reshape(R, H)) if need_w else None
+    inv = inverse_perm.contiguous()
+    w = None if weights is None else weights.contiguous()
+    if out is None:
+        out = UnsortGradients(torch.empty(y_shape, dtype=g.dtype, device=dev) if need_y else None,
+                              torch.empty((T, K), dtype=torch.float32, device=dev) if need_w else None)
+    else:
+        if (out.rows is not None) != need_y or (out.weights is not None) != need_w:
+            raise ValueError("unsort_tokens_backward: out must hold the gradients that are asked for")
+        if need_y:
+            check_out("unsort_tokens_backward", out.rows, y_shape, g.dtype, dev, g, y2, inv, w)
+            if out.rows.data_ptr() % 16:
+                raise ValueError("unsort_tokens_backward: out.rows must be 16-byte aligned")
+        if need_w:
+            check_out("unsort_tokens_backward", out.weights, (T, K), torch.float32, dev, g, y2, inv, w)
+    n_rows = None if offsets is None else offsets.data_ptr() + 4 * (offsets.numel() - 1)
+    call(dev, _cabi.lib().moe_rd_unsort_tokens_backward, T, H, K, ROW_DTYPE[g.dtype], _ptr(g), _ptr(y2), R, _ptr(inv), _ptr(w),
+         n_rows, _ptr(out.rows), _ptr(out.weights))
+    return out
+
+
+def unsort_tokens_backward(grad_out: torch.Tensor, y: torch.Tensor, inverse_perm: torch.Tensor,
+                           weights: Optional[torch.Tensor] = None, *, offsets: Optional[torch.Tensor] = None,
+                           need_rows: bool = True, need_weights: Optional[bool] = None,
+                           out: Optional[UnsortGradients] = None) -> UnsortGradients:
+    """Gradients of ``unsort_tokens`` for ``grad_out`` [T, H]: of the rows of ``y`` (the type of y) and of ``weights``
+    (fp32, added in a fixed order; asked for by default where weights are given).  The gradient of ``shared`` is
+    ``grad_out`` itself.  Rows of y that no pair has (with ``offsets``: those from ``offsets[-1]`` on) get a zero
+    gradient.  ``out`` takes the result of an earlier call of the same sizes."""
+    need_weights = weights is not None if need_weights is None else need_weights
+    _check_unsort("unsort_tokens_backward", y, inverse_perm, weights, grad_out)
+    _check_offsets("unsort_tokens_backward", offsets)
+    if not (need_rows or need_weights):
+        raise ValueError("unsort_tokens_backward: no gradient is asked for")
+    check_device("unsort_tokens_backward", grad_out, y, inverse_perm, weights, offsets)
+    return _unsort_backward(grad_out, y, y.shape, inverse_perm, weights, offsets, need_rows, need_weights, out)
+
+
+# --- routing weights -------------------------------------------------------------------------------------------------
+def _check_weights(name, logits, expert_ids, bias, bias_mode, score_fn):
+    if logits.dtype != torch.float32:
+        raise TypeError(f"{name}: logits must be float32")
+    T, K = _check_ids(name, expert_ids)
+    if logits.dim() != 2 or logits.shape[0] != T or logits.shape[1] < 1:
+        raise ValueError(f"{name}: logits must be [T, E] for the T = {T} tokens of expert_ids")
+    if score_fn not in SCORE_FN:
+        raise ValueError(f"{name}: score_fn must be one of {tuple(SCORE_FN)}")
+    if bias_mode not in BIAS_MODES:
+        raise ValueError(f"{name}: bias_mode must be one of {BIAS_MODES}")
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != logits.shape[1]):
+        raise ValueError(f"{name}: bias must be a float32 tensor of E elements")
+    if bias is not None and wants_grad(bias):
+        raise ValueError(f"{name}: bias is a constant here; add a learned bias to the logits")
+
+
+def _weights_call(entry, logits, expert_ids, bias, bias_mode, score_fn, renorm, routed_scale, norm_min, *rest):
+    T, E = logits.shape
+    lg = logits.contiguous()
+    ids = expert_ids.contiguous()
+    b = None if bias is None else bias.contiguous()
+    call(logits.device, entry, T, E, ids.shape[1], SCORE_FN[score_fn], int(bool(renorm)), float(routed_scale), float(norm_min), _ptr(lg),
+         _ptr(ids), _ptr(b) if bias_mode == "logit" else None, _ptr(b) if bias_mode == "select_and_weight" else None, *map(_ptr, rest))
+
+
+class _RoutingWeights(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, expert_ids, bias, config):
+        out = torch.empty(expert_ids.shape, dtype=torch.float32, device=logits.device)
+        _weights_call(_cabi.lib().moe_rd_routing_weights, logits, expert_ids, bias, *config, out)
+        ctx.save_for_backward(logits, expert_ids, bias)
+        ctx.config = config
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        _not_while_capturing("routing_weights", "routing_weights on detached logits and routing_weights_backward")
+        logits, expert_ids, bias = ctx.saved_tensors
+        out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
+        _weights_call(_cabi.lib().moe_rd_routing_weights_backward, logits, expert_ids, bias, *ctx.config, grad.contiguous(), out)
+        return out, None, None, None
+
+
+def routing_weights(logits: torch.Tensor, expert_ids: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                    score_fn: str = "softmax", bias_mode: str = "select", renorm: bool = True, routed_scale: float = 1.0,
+                    norm_min: float = 1e-20, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The combine weights [T, K] of the experts ``expert_ids`` as a function of the router's ``logits`` [T, E] fp32.
+
+    The keywords are those of ``route_dispatch``, whose ``combine_weights`` these are (within rounding) for the ids that it
+    chose; a bias that is for selection only ("select") has no part in them.  Slots whose id is outside [0, E) have
+    weight 0 and no part in the sum.  Differentiable in ``logits`` (ids and bias are constants): with
+    ``logits = x @ gate_weight`` it carries the gradient of the weights to the router.
+    """
+    _check_weights("routing_weights", logits, expert_ids, bias, bias_mode, score_fn)
+    dev = check_device("routing_weights", logits, expert_ids, bias)
+    config = (bias_mode, score_fn, renorm, routed_scale, norm_min)
+    if wants_grad(logits):
+        if out is not None:
+            raise ValueError("routing_weights: out cannot be given where a gradient is required")
+        _not_while_capturing("routing_weights", "routing_weights on detached logits and routing_weights_backward")
+        return _RoutingWeights.apply(logits, expert_ids, bias, config)
+    if out is None:
+        out = torch.empty(expert_ids.shape, dtype=torch.float32, device=dev)
+    else:
+        check_out("routing_weights", out, expert_ids.shape, torch.float32, dev, logits, expert_ids, bias)
+    _weights_call(_cabi.lib().moe_rd_routing_weights, logits, expert_ids, bias, *config, out)
+    return out
+
+
+def routing_weights_backward(grad_weights: torch.Tensor, logits: torch.Tensor, expert_ids: torch.Tensor,
+                             bias: Optional[torch.Tensor] = None, *, score_fn: str = "softmax", bias_mode: str = "select",
+                             renorm: bool = True, routed_scale: float = 1.0, norm_min: float = 1e-20,
+                             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient [T, E] fp32 of ``routing_weights`` with respect to the logits, for ``grad_weights`` [T, K] fp32.  Where
+    the sum of the chosen scores is below ``norm_min`` it has no part in the gradient; a token without any valid id gets
+    zeros."""
+    _check_weights("routing_weights_backward", logits, expert_ids, bias, bias_mode, score_fn)
+    if grad_weights.dtype != torch.float32 or grad_weights.shape != expert_ids.shape:
+        raise ValueError("routing_weights_backward: grad_weights must be a float32 tensor like expert_ids")
+    dev = check_device("routing_weights_backward", logits, grad_weights, expert_ids, bias)
+    grad = grad_weights.contiguous()
+    if out is None:
+        out = torch.empty(logits.shape, dtype=torch.float32, device=dev)
+    else:
+        check_out("routing_weights_backward", out, logits.shape, torch.float32, dev, logits, expert_ids, bias, grad)
+    _weights_call(_cabi.lib().moe_rd_routing_weights_backward, logits, expert_ids, bias, bias_mode, score_fn, renorm, routed_scale,
+                  norm_min, grad, out)
+    return out

@@ -388,6 +388,109 @@ int moe_rd_gemm_plan(const int32_t* offsets, int32_t E, const void* a_rows, int6
 int moe_rd_expert_stats(const int32_t* offsets, const float* row_weight, int32_t E,
                         float* weight_sum, float* mean_weight, float* load, void* stream);
 
+/* Element types of the rows that the entry points below take. */
+enum { MOE_RD_T_BF16 = 0, MOE_RD_T_FP16 = 1, MOE_RD_T_F32 = 2 };
+
+/*
+ * Tokens sorted by expert, for expert ids that the caller already has (a router
+ * of its own, a replayed routing, the backward of a recomputed layer):
+ *   rows[inverse_perm[t,k], :] = x[t, :]     for every pair (t,k) that has a row
+ * in the order of moe_rd_route_dispatch: experts ascending, inside an expert the
+ * stable (token, slot) order, pairs past `capacity` rows of their expert (0 = no
+ * limit) without a row.  A pair whose id is outside [0, E) has no expert and no
+ * row (a padded token has K such pairs); the same expert may occur twice among a
+ * token's ids.  inverse_perm is -1 for a pair without a row.
+ *   x [T,H], rows [out_rows,H]   elements of type `dtype` (MOE_RD_T_*), 16-byte
+ *                                aligned, H * element size a multiple of 16
+ *   expert_ids [T,K], inverse_perm [T,K], offsets [E+1], row_token [out_rows]
+ *   (token of every row), counts [E] (pairs per expert before dropping, or NULL)
+ * out_rows: at least T*K, or E*capacity where that is less.  Every output is
+ * written whole: rows behind offsets[E] become zero, with row_token -1.
+ * E <= 256, K <= 32 (K may exceed E).  Workspace: moe_rd_sort_workspace_bytes
+ * bytes, 256-byte aligned; nothing in it has to be initialised.  May be recorded
+ * into a CUDA graph.
+ */
+int moe_rd_sort_workspace_bytes(int64_t T, int32_t E, int32_t K, size_t* bytes);
+int moe_rd_sort_tokens(int64_t T, int32_t H, int32_t E, int32_t K, int32_t dtype, int64_t capacity,
+                       int64_t out_rows, const void* x, const int32_t* expert_ids, void* rows,
+                       int32_t* offsets, int32_t* inverse_perm, int32_t* row_token, int32_t* counts,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The way back, for rows of any type:
+ *   out[t,:] = shared[t,:] + sum_k weights[t,k] * y[inverse_perm[t,k],:]
+ * as moe_rd_combine computes it (fp32 accumulation from the shared row, slots in
+ * order, one rounding).  weights NULL: every weight is 1, which makes the call
+ * the gradient of moe_rd_sort_tokens (y = gradient of rows, out = gradient of
+ * x).  shared may be NULL.  A row index outside [0, y_rows) is a pair without a
+ * row: whatever its weight is, it contributes nothing.
+ */
+int moe_rd_unsort_tokens(int64_t T, int32_t H, int32_t K, int32_t dtype, const void* y, int64_t y_rows,
+                         const int32_t* inverse_perm, const float* weights, const void* shared,
+                         void* out, void* stream);
+
+/*
+ * Gradients of moe_rd_unsort_tokens, for grad_out [T,H]:
+ *   grad_y[inverse_perm[t,k],:] = weights[t,k] * grad_out[t,:]     (one rounding)
+ *   grad_weights[t,k] = sum_h grad_out[t,h] * y[inverse_perm[t,k],h]   (fp32, in
+ *                       a fixed order; 0 for a pair without a row)
+ * (the gradient of `shared` is grad_out itself).  Either output may be NULL; y is
+ * read for grad_weights only.  Every row index may occur once at most, as in what
+ * moe_rd_sort_tokens and moe_rd_route_dispatch return.  grad_y is written whole:
+ * n_rows is a DEVICE int32 (offsets[E]) from which on the rows of y are nobody's
+ * and their gradient is zero; with n_rows NULL all of grad_y is cleared first.
+ */
+int moe_rd_unsort_tokens_backward(int64_t T, int32_t H, int32_t K, int32_t dtype, const void* grad_out,
+                                  const void* y, int64_t y_rows, const int32_t* inverse_perm,
+                                  const float* weights, const int32_t* n_rows, void* grad_y,
+                                  float* grad_weights, void* stream);
+
+/*
+ * The combine weights of chosen experts as a function of the router's logits,
+ * and its gradient: with s = softmax(z) or sigmoid(z), z = logits (+ logit_bias),
+ * and u_k = s[expert_ids[t,k]] (+ select_bias of that expert, where it is given:
+ * the weight_from_key form of moe_rd_params),
+ *   weights[t,k] = routed_scale * u_k / max(sum_j u_j, norm_min)   (renorm), or
+ *                  routed_scale * u_k
+ * moe_rd_routing_weights_backward: grad_logits [T,E] = the gradient of
+ * sum(grad_weights * weights) with respect to the logits; the ids and biases are
+ * constants.  Where sum_j u_j < norm_min the sum has no gradient.  logits [T,E],
+ * fp32; a slot whose id is outside [0, E) has weight 0 and no part in the sums; a
+ * token without any valid id gets a zero gradient whatever its logits are.
+ */
+int moe_rd_routing_weights(int64_t T, int32_t E, int32_t K, int32_t score_fn, int32_t renorm,
+                           float routed_scale, float norm_min, const float* logits,
+                           const int32_t* expert_ids, const float* logit_bias, const float* select_bias,
+                           float* weights, void* stream);
+int moe_rd_routing_weights_backward(int64_t T, int32_t E, int32_t K, int32_t score_fn, int32_t renorm,
+                                    float routed_scale, float norm_min, const float* logits,
+                                    const int32_t* expert_ids, const float* logit_bias,
+                                    const float* select_bias, const float* grad_weights,
+                                    float* grad_logits, void* stream);
+
+/*
+ * Products of few rows with 4-bit expert weights, the expert layer of a decode
+ * step: for every expert e and every row r in [offsets[e], offsets[e+1])
+ *   out[r,n] = sum_k x[r,k] * (q[e,n,k] - zero[e,n,k/group]) * scale[e,n,k/group]
+ * x [rows,K] and out [rows,N] bf16 or fp16 (dtype; fp32 is not offered), scales in
+ * the same type, q in 0..15, zero in 0..15 (8 where `zeros` is NULL).  offsets
+ * NULL: one expert (E = 1) that has every row.  Rows before offsets[0] and from
+ * offsets[E] on become zero.  The products of a group are added in fp32 and
+ * scaled in fp32; the result is rounded once.  Every weight of an expert that has
+ * rows is read once per eight of its rows, so the call is meant for few rows per
+ * expert; it is right for any number.
+ * K % group == 0, group % 32 == 0; x and out 16-byte aligned.  The weights are laid
+ * out in tiles of 16 outputs x 128 inputs (with C = ceil(K/128), B = ceil(N/16),
+ * G = K/group), zero-padded:
+ *   weight [E][B][C][1024 bytes]: half h (outputs 16b + 8h + 0..7), lane l = 4*r + j
+ *     (r: output inside the half), word i (16 bytes a lane): the eight inputs
+ *     128c + 32i + 8j + 0..7 of that output; input 2p in bits 4p.., input 2p+1 in bits 16+4p..
+ *   scales [E][B][G][16], zeros [E][B][G][16] (one byte each)
+ */
+int moe_rd_expert_matvec_w4(int64_t rows, int32_t N, int32_t K, int32_t E, int32_t group, int32_t dtype,
+                            const void* x, const void* weight, const void* scales, const uint8_t* zeros,
+                            const int32_t* offsets, void* out, void* stream);
+
 /* Kernels this library launched since it was loaded (all threads). */
 int64_t moe_rd_launch_count(void);
 

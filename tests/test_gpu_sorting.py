@@ -1,0 +1,375 @@
+"""Sorting tokens by expert and back, with weights, and the gradients, against plain statements in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import moe_rd
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+HALF_STEP = {"bf16": 2.0 ** -8, "fp16": 2.0 ** -11, "fp32": 2.0 ** -24}
+TINY = {"bf16": 2.0 ** -134, "fp16": 2.0 ** -25, "fp32": 2.0 ** -150}   # half of the smallest number of the type
+
+
+def places(ids, E, capacity):
+    """A walk over the pairs: row of every pair, offsets, counts, token of every row."""
+    T, K = ids.shape
+    lists = [[] for _ in range(E)]
+    counts = np.zeros(E, np.int32)
+    for t in range(T):
+        for k in range(K):
+            e = int(ids[t, k])
+            if 0 <= e < E:
+                counts[e] += 1
+                if capacity == 0 or len(lists[e]) < capacity:
+                    lists[e].append((t, k))
+    inv = np.full((T, K), -1, np.int32)
+    offsets = np.zeros(E + 1, np.int32)
+    token = []
+    for e in range(E):
+        for t, k in lists[e]:
+            inv[t, k] = len(token)
+            token.append(t)
+        offsets[e + 1] = len(token)
+    return inv, offsets, counts, np.array(token, np.int64)
+
+
+def ids_of(T, K, E, kind, seed=0):
+    g = torch.Generator().manual_seed(seed + 7 * T + K)
+    ids = torch.randint(0, E, (T, K), generator=g, dtype=torch.int32)
+    if kind == "padded":
+        ids[torch.rand(T, generator=g) < 0.4] = -1
+    elif kind == "one expert":
+        ids[:] = E - 1
+    elif kind == "none":
+        ids[:] = -1
+    elif kind == "stray":
+        ids[torch.rand(T, K, generator=g) < 0.2] = E
+        ids[torch.rand(T, K, generator=g) < 0.1] = -2 ** 31
+        ids[torch.rand(T, K, generator=g) < 0.1] = 2 ** 31 - 1
+    return ids
+
+
+SORT_CASES = [
+    # T, K, E, H, dtype, capacity, ids
+    (1, 8, 256, 7168, "bf16", 0, "random"),
+    (1, 1, 1, 8, "bf16", 0, "random"),
+    (3, 2, 5, 4, "fp32", 0, "padded"),
+    (7, 3, 60, 264, "fp16", 1, "random"),
+    (128, 8, 256, 1024, "bf16", 0, "random"),     # 1024 pairs: the last size of the one-kernel form
+    (129, 8, 256, 1024, "bf16", 0, "random"),     # the first of the batch form
+    (1025, 1, 7, 20, "fp32", 100, "padded"),
+    (33, 32, 4, 72, "fp16", 0, "random"),         # more ids than experts: the same expert several times per token
+    (64, 32, 256, 40, "bf16", 3, "stray"),
+    (2047, 2, 8, 136, "bf16", 300, "one expert"),
+    (2049, 2, 8, 516, "fp32", 0, "stray"),        # one token into a second group of counting tiles
+    (40, 4, 16, 64, "bf16", 0, "none"),
+    (600, 4, 16, 64, "fp16", 2, "none"),
+    (5000, 6, 160, 520, "fp16", 200, "padded"),
+]
+
+
+@pytest.mark.parametrize("T,K,E,H,dtype,capacity,kind", SORT_CASES)
+def test_sort_is_exact(T, K, E, H, dtype, capacity, kind):
+    ids = ids_of(T, K, E, kind)
+    x = torch.randn(T, H, generator=torch.Generator().manual_seed(T)).to(DT[dtype])
+    x.view(-1)[::97] = float("nan")
+    x.view(-1)[1::89] = float("inf")
+    inv, offsets, counts, token = places(ids.numpy(), E, capacity)
+    for run in range(2):  # a second call into the buffers of the first, which hold other things by then
+        out = None
+        if run:
+            for t in got:
+                t.view(torch.uint8).fill_(0x55)
+            out = got
+        got = moe_rd.sort_tokens(x.cuda(), ids.cuda(), E, capacity=capacity, out=out)
+        np.testing.assert_array_equal(got.inverse_perm.cpu().numpy(), inv)
+        np.testing.assert_array_equal(got.offsets.cpu().numpy(), offsets)
+        np.testing.assert_array_equal(got.counts.cpu().numpy(), counts)
+        R = min(T * K, E * capacity) if capacity else T * K
+        assert got.rows.shape == (R, H) and got.row_token.shape == (R,)
+        want_token = np.full(R, -1, np.int32)
+        want_token[:len(token)] = token
+        np.testing.assert_array_equal(got.row_token.cpu().numpy(), want_token)
+        want = torch.zeros(R, H, dtype=x.dtype)
+        want[:len(token)] = x[torch.from_numpy(token)]
+        assert torch.equal(got.rows.cpu().view(torch.uint8), want.view(torch.uint8))  # bit copies, NaN included
+
+
+def test_sort_of_no_tokens_and_of_views():
+    e = torch.zeros((0, 2), dtype=torch.int32).cuda()
+    got = moe_rd.sort_tokens(torch.zeros(0, 64, dtype=torch.bfloat16).cuda(), e, 4)
+    assert got.rows.shape == (0, 64) and got.offsets.tolist() == [0] * 5 and got.counts.tolist() == [0] * 4
+    base = torch.randn(50, 2 * 128 + 1).cuda()
+    ids = ids_of(20, 4, 6, "padded").cuda()
+    for x in (base[:20, 1:129], base[:40:2, ::2][:, :128], base[:20, :128].reshape(4, 5, 128), base.t()[:20, :48]):
+        H = x.shape[-1]
+        wide = torch.cat([ids, ids], 1)[:, ::2]  # a strided view of ids
+        a = moe_rd.sort_tokens(x, wide, 6)
+        b = moe_rd.sort_tokens(x.reshape(20, H).clone(), wide.clone(), 6)
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_sort_agrees_with_route_dispatch():
+    """The ids, capacity and rows of a routed batch, sorted again: the same places."""
+    from moe_rd import workloads
+    t, kw = workloads.make("c3", T=3000, H=512)
+    r = moe_rd.route_dispatch(t["x"].cuda(), t["w"].cuda(), t["bias"].cuda(), return_row_meta=True, **kw)
+    s = moe_rd.sort_tokens(t["x"].cuda(), r.expert_ids, 128, capacity=kw["capacity"])
+    live = int(r.offsets[-1])
+    assert torch.equal(s.offsets, r.offsets) and torch.equal(s.inverse_perm, r.inverse_perm) and torch.equal(s.counts, r.counts)
+    assert torch.equal(s.rows[:live], r.permuted[:live]) and torch.equal(s.row_token[:live], r.row_token[:live])
+
+
+def random_places(T, K, R, seed, missing=0.2):
+    """Every row of 0..n-1 once, in a random order; pairs without a row in between."""
+    g = torch.Generator().manual_seed(seed)
+    has = torch.rand(T * K, generator=g) >= missing
+    n = min(int(has.sum()), R)
+    at = torch.nonzero(has)[:, 0][:n]
+    inv = torch.full((T * K,), -1, dtype=torch.int32)
+    inv[at] = torch.randperm(n, generator=g).to(torch.int32)
+    return inv.reshape(T, K), n
+
+
+UNSORT_CASES = [
+    # T, K, H, dtype, weighted, shared
+    (1, 8, 7168, "bf16", True, True),
+    (1, 1, 8, "bf16", False, False),
+    (5, 3, 4, "fp32", True, False),
+    (70, 2, 264, "fp16", True, True),
+    (33, 8, 1040, "bf16", False, True),
+    (300, 20, 264, "bf16", True, False),
+    (129, 10, 132, "fp32", False, False),
+    (2000, 4, 520, "fp16", True, False),
+    (777, 6, 2056, "bf16", True, False),
+    (64, 32, 40, "fp16", True, True),
+]
+
+
+def unsort_inputs(T, K, H, dtype, seed=1, missing=0.2):
+    R = T * K
+    g = torch.Generator().manual_seed(seed + T)
+    inv, n = random_places(T, K, R, seed, missing)
+    y = torch.randn(R, H, generator=g).to(DT[dtype])
+    w = torch.randn(T, K, generator=g)
+    sh = torch.randn(T, H, generator=g).to(DT[dtype])
+    return y, inv, w, sh, n
+
+
+def unsort64(y, inv, w, sh):
+    """The formula in 64 bits, and the sum of the terms' magnitudes."""
+    T, K = inv.shape
+    rows = y.double()[inv.clamp(min=0).long()] * (inv >= 0)[..., None]
+    terms = rows if w is None else rows * (w.double() * (inv >= 0))[..., None]
+    out, mag = terms.sum(1), terms.abs().sum(1)
+    if sh is not None:
+        out, mag = out + sh.double(), mag + sh.double().abs()
+    return out, mag
+
+
+@pytest.mark.parametrize("T,K,H,dtype,weighted,shared", UNSORT_CASES)
+def test_unsort(T, K, H, dtype, weighted, shared):
+    y, inv, w, sh, _ = unsort_inputs(T, K, H, dtype)
+    w, sh = w if weighted else None, sh if shared else None
+    want, mag = unsort64(y, inv, w, sh)
+    if weighted:
+        w = torch.where(inv < 0, torch.full_like(w, float("nan")), w)   # a pair without a row has no say
+    got = moe_rd.unsort_tokens(y.cuda(), inv.cuda(), None if w is None else w.cuda(), None if sh is None else sh.cuda())
+    # K fused multiply-adds in 32 bits, each within 2^-24 of a partial sum that the magnitudes bound, then one rounding
+    low = K * 2.0 ** -24 * mag * (1 + K * 2.0 ** -24)
+    bound = low + HALF_STEP[dtype] * (want.abs() + low) + TINY[dtype]
+    assert ((got.cpu().double() - want).abs() <= bound).all()
+
+
+def test_unsort_ignores_rows_out_of_range():
+    y = torch.randn(10, 64).cuda()
+    inv = torch.tensor([[0, 10], [2 ** 31 - 1, -2 ** 31], [9, -1]], dtype=torch.int32).cuda()
+    w = torch.ones(3, 2).cuda()
+    got = moe_rd.unsort_tokens(y, inv, w)
+    assert torch.equal(got, torch.stack([y[0], torch.zeros_like(y[0]), y[9]]))
+    none = moe_rd.unsort_tokens(y[:0], inv, w, y[:3])
+    assert torch.equal(none, y[:3])
+    # fp32 rows and weights of 1: equal to no weights at all
+    assert torch.equal(moe_rd.unsort_tokens(y, inv), got)
+
+
+def test_unsort_equals_combine():
+    y, inv, w, sh, _ = unsort_inputs(400, 8, 512, "bf16")
+    a = moe_rd.unsort_tokens(y.cuda(), inv.cuda(), w.cuda(), sh.cuda())
+    assert torch.equal(a, moe_rd.combine(y.cuda(), inv.cuda(), w.cuda(), sh.cuda()))
+
+
+@pytest.mark.parametrize("T,K,H,dtype,weighted,shared", UNSORT_CASES)
+@pytest.mark.parametrize("with_offsets", [True, False])
+def test_unsort_gradients(T, K, H, dtype, weighted, shared, with_offsets):
+    y, inv, w, _, n = unsort_inputs(T, K, H, dtype, seed=3)
+    g = torch.randn(T, H, generator=torch.Generator().manual_seed(9)).to(DT[dtype])
+    offsets = torch.tensor([0, n], dtype=torch.int32).cuda() if with_offsets else None
+    want_y = torch.zeros(T * K, H, dtype=torch.float64)
+    has = inv >= 0
+    each = (w.double()[..., None] if weighted else 1.0) * g.double()[:, None, :].expand(T, K, H)
+    want_y[inv[has].long()] = each[has]
+    rows = y.double()[inv.clamp(min=0).long()] * has[..., None]
+    want_w = (rows * g.double()[:, None, :]).sum(2)
+    mag_w = (rows * g.double()[:, None, :]).abs().sum(2)
+    wc = w.cuda() if weighted else None
+    got = moe_rd.unsort_tokens_backward(g.cuda(), y.cuda(), inv.cuda(), wc, offsets=offsets, need_weights=True)
+    # one product in 32 bits, then one rounding (no rounding at all without weights)
+    bound = want_y.abs() * (HALF_STEP[dtype] + 2.0 ** -24 * (1 + HALF_STEP[dtype])) + TINY[dtype]
+    assert ((got.rows.cpu().double() - want_y).abs() <= bound).all()
+    # a lane adds at most ceil(H / 32) products, 5 + 7 additions join lanes and warps
+    assert ((got.weights.cpu().double() - want_w).abs() <= (H / 32 + 9 + 12) * 2.0 ** -24 * mag_w).all()
+    assert (got.weights.cpu()[~has] == 0).all()
+    # the same bits again, into the buffers of the first call; and each gradient alone
+    first = [t.clone() for t in got]
+    for t in got:
+        t.fill_(float("nan"))
+    again = moe_rd.unsort_tokens_backward(g.cuda(), y.cuda(), inv.cuda(), wc, offsets=offsets, need_weights=True, out=got)
+    assert again is got and all(torch.equal(p, q) for p, q in zip(first, again))
+    assert torch.equal(moe_rd.unsort_tokens_backward(g.cuda(), y.cuda(), inv.cuda(), wc, offsets=offsets, need_weights=False).rows, first[0])
+    assert torch.equal(moe_rd.unsort_tokens_backward(g.cuda(), y.cuda(), inv.cuda(), wc, need_rows=False, need_weights=True).weights,
+                       first[1])
+
+
+def test_gradients_of_padded_and_empty_batches():
+    z = torch.zeros(0, 2, dtype=torch.int32).cuda()
+    got = moe_rd.unsort_tokens_backward(torch.zeros(0, 64).cuda(), torch.randn(5, 64).cuda(), z, need_weights=True)
+    assert torch.equal(got.rows, torch.zeros(5, 64).cuda()) and got.weights.shape == (0, 2)
+    inv = torch.full((9, 3), -1, dtype=torch.int32).cuda()
+    nan = torch.full((9, 64), float("nan")).cuda()
+    got = moe_rd.unsort_tokens_backward(nan, torch.randn(27, 64).cuda(), inv, torch.ones(9, 3).cuda(),
+                                        offsets=torch.zeros(2, dtype=torch.int32).cuda())
+    assert torch.equal(got.rows, torch.zeros(27, 64).cuda()) and torch.equal(got.weights, torch.zeros(9, 3).cuda())
+
+
+@pytest.mark.parametrize("T,K,E,H,capacity", [(37, 3, 5, 20, 0), (300, 4, 8, 64, 90)])
+def test_autograd_against_differences(T, K, E, H, capacity):
+    """Sort, a factor per row, and back: the gradients are those of the formula, and agree with differences of it
+    along a random direction.  The formula is linear in each argument, so a central difference has no error of its own."""
+    g = torch.Generator().manual_seed(T)
+    ids = ids_of(T, K, E, "padded", 5)
+    inv, _, _, token = places(ids.numpy(), E, capacity)
+    R = min(T * K, E * capacity) if capacity else T * K
+    x = torch.randn(T, H, generator=g)
+    w = torch.rand(T, K, generator=g)
+    sh = torch.randn(T, H, generator=g)
+    f = torch.randn(R, H, generator=g)
+    go = torch.randn(T, H, generator=g)
+    invt = torch.from_numpy(inv)
+
+    def loss64(x, w, sh):
+        rows = torch.zeros(R, H, dtype=torch.float64)
+        rows[:len(token)] = x[torch.from_numpy(token)]
+        return (unsort64(rows * f.double(), invt, w, sh)[0] * go.double()).sum()
+
+    leaves = [t.cuda().requires_grad_() for t in (x, w, sh)]
+    s = moe_rd.sort_tokens(leaves[0], ids.cuda(), E, capacity=capacity)
+    assert s.rows.requires_grad and not s.offsets.requires_grad
+    out = moe_rd.unsort_tokens(s.rows * f.cuda(), s.inverse_perm, leaves[1], leaves[2], offsets=s.offsets)
+    out.backward(go.cuda())
+    ref = [t.double().requires_grad_() for t in (x, w, sh)]
+    loss64(*ref).backward()
+    for got, want in zip(leaves, ref):
+        # at most H + K + 4 roundings of 2^-24 on sums whose terms are below 30 in magnitude here
+        err = (got.grad.cpu().double() - want.grad).abs().max()
+        assert err <= (H + K + 4) * 2.0 ** -24 * 30 * K
+    for i, base in enumerate((x, w, sh)):
+        d = torch.randn(base.shape, generator=g).double()
+        args = [t.double() for t in (x, w, sh)]
+        up, down = list(args), list(args)
+        up[i], down[i] = args[i] + d, args[i] - d
+        diff = (loss64(*up) - loss64(*down)) / 2
+        along = (leaves[i].grad.cpu().double() * d).sum()
+        assert (along - diff).abs() <= (H + K + 4) * 2.0 ** -24 * 30 * K * d.abs().sum()
+
+
+def test_a_training_layer_end_to_end():
+    """route_dispatch's ids, routing_weights, sort_tokens, expert products and unsort_tokens: the gradients of the tokens,
+    the gate, the experts and the shared branch against the same layer in 64 bits."""
+    T, H, E, K, N = 200, 128, 8, 3, 128
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(T, H, generator=g).to(torch.bfloat16).float()
+    wg = torch.randn(H, E, generator=g) * 0.1
+    we = torch.randn(E, H, N, generator=g) * 0.1
+    go = torch.randn(T, N, generator=g)
+    capacity = 90
+
+    leaves = [t.cuda().requires_grad_() for t in (x, wg, we)]
+    logits = leaves[0] @ leaves[1]
+    r = moe_rd.route_dispatch(x.cuda().to(torch.bfloat16), None, top_k=K, given_logits=logits.detach(), capacity=capacity,
+                              scatter_impl="none")
+    w = moe_rd.routing_weights(logits, r.expert_ids)
+    torch.testing.assert_close(w.detach(), r.combine_weights, rtol=2e-6, atol=0)   # the same function, other roundings
+    s = moe_rd.sort_tokens(leaves[0], r.expert_ids, E, capacity=capacity)
+    assert torch.equal(s.inverse_perm, r.inverse_perm)
+    o = s.offsets.tolist()
+    y = torch.cat([s.rows[o[e]:o[e + 1]] @ leaves[2][e] for e in range(E)] + [s.rows[o[E]:] @ leaves[2][0]])
+    out = moe_rd.unsort_tokens(y, s.inverse_perm, w, leaves[0], offsets=s.offsets)
+    out.backward(go.cuda())
+
+    ids, inv = r.expert_ids.cpu().long(), r.inverse_perm.cpu()
+    ref = [t.double().requires_grad_() for t in (x, wg, we)]
+    z = torch.softmax(ref[0] @ ref[1], 1).gather(1, ids)
+    wr = z / z.sum(1, keepdim=True) * (inv >= 0)
+    yr = torch.einsum("th,tkhn->tkn", ref[0], ref[2][ids])
+    want = (wr[..., None] * yr).sum(1) + ref[0]
+    want.backward(go.double())
+    assert (out.detach().cpu().double() - want.detach()).abs().max() <= 1e-4 * want.detach().abs().max()
+    for got, exact in zip(leaves, ref):
+        # sums of at most T * K * H products in 32 bits; their roundings add up like a random walk: 2^-24 * sqrt(76800) < 2e-5
+        assert (got.grad.cpu().double() - exact.grad).norm() <= 2e-5 * exact.grad.norm()
+
+
+def test_graph_replay_and_streams():
+    """The plain functions recorded into a graph and replayed on new inputs; and run on another stream."""
+    T, K, E, H = 700, 4, 16, 256
+    x, y, ids = torch.randn(T, H).cuda(), torch.randn(T * K, H).cuda(), ids_of(T, K, E, "padded").cuda()
+    w, g = torch.rand(T, K).cuda(), torch.randn(T, H).cuda()
+
+    def step():
+        s = moe_rd.sort_tokens(x, ids, E)
+        few = moe_rd.sort_tokens(x[:9], ids[:9], E)
+        out = moe_rd.unsort_tokens(y, s.inverse_perm, w)
+        grads = moe_rd.unsort_tokens_backward(g, y, s.inverse_perm, w, offsets=s.offsets)
+        dx = moe_rd.unsort_tokens(grads.rows, s.inverse_perm)
+        return (*s, *few, out, *grads, dx)
+
+    step()
+    torch.cuda.synchronize()
+    pool = torch.cuda.graph_pool_handle()
+    graphs = []
+    for _ in range(2):  # two graphs that share one memory pool, replayed in turn
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            res = step()
+        graphs.append((graph, res))
+    x.normal_()
+    y.normal_()
+    ids.copy_(ids_of(T, K, E, "stray", 3))
+    for graph, res in graphs:
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in res]
+        assert all(torch.equal(a, b) for a, b in zip(kept, step()))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(there, step()))
+
+
+def test_autograd_is_refused_while_capturing():
+    x = torch.randn(8, 64, device="cuda", requires_grad=True)
+    y = torch.randn(16, 64, device="cuda", requires_grad=True)
+    ids = ids_of(8, 2, 4, "random").cuda()
+    inv = moe_rd.sort_tokens(x.detach(), ids, 4).inverse_perm
+    torch.cuda.synchronize()
+    for fn in (lambda: moe_rd.sort_tokens(x, ids, 4), lambda: moe_rd.unsort_tokens(y, inv)):
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="not recorded into a CUDA graph"):
+            with torch.cuda.graph(graph):
+                fn()
+    assert torch.equal(moe_rd.sort_tokens(x, ids, 4).inverse_perm, inv)
