@@ -1,21 +1,32 @@
 // Products of few rows with 4-bit expert weights (moe_rd_expert_matvec_w4):
 //   out[r,n] = sum_groups scale[n,group] * sum_{k in group} x[r,k] * (q[n,k] - zero[n,group])
 //
-// Reading the weights (half a byte each) of the experts that have rows is nearly all the traffic, so HBM is the floor.
-// A product on the CUDA cores would need one FMA per weight and row; from three rows on that is slower than the
-// memory.  So the weights go through the warp's matrix instruction (mma m16n8k16: 16 outputs x 16 inputs times 8
-// rows of x): q - zero is an integer in -15..15, exact in bf16 and fp16, and the group's scale multiplies the fp32 sum
-// of the group afterwards, so nothing is rounded below 32 bits before the result is.
+// Reading the weights (half a byte each) of the experts that have rows is nearly all the traffic, so HBM is the floor:
+// 43 bytes, 87 weights, per nanosecond and SM.  A product on the CUDA cores would need one FMA per weight and row; from
+// two rows on that is slower than the memory.  So the weights go through the warp's matrix instruction (mma m16n8k16: 16
+// outputs x 16 inputs times 8 rows of x), and what has to be kept small is the number of instructions that turn 4-bit
+// integers into its operands:
 //
-// The weight tile of 16 outputs x 128 inputs is 1 KB, stored so that a lane's two 16-byte loads are its operand
-// fragments: word i holds the eight inputs 32i + 8j.. of one output, the pair (2p, 2p+1) in nibbles p of its two
-// halves, so that (w >> 4p) & 0x000f000f is a pair of integers; with the exponent bits of 128 (bf16) or 1024 (fp16)
-// or'ed in it is a pair of floats 128 + q (1024 + q), from which 128 + zero (1024 + zero) is subtracted exactly.
-// Every 16 inputs of one instruction lie inside one block of 32, so groups of 32, 64, 96, ... inputs work alike.
+// * A tile of 32 outputs x 128 inputs is 2 KB, stored so that a lane's 16-byte loads are its operand fragments: word i
+//   holds the eight inputs 32i + 8j.. of one output, the pair (2p, 2p+1) in its two halves.
+// * bf16: the four bits of pair p are the topmost mantissa bits of each half once the word is rotated by 4p; with the
+//   exponent of 16 that is the pair of numbers 16 + q, one rotation and one LOP3 for two weights.  The matrix
+//   instruction multiplies those, and (16 + zero) * sum of x over the group is subtracted from the group's fp32 sum; the
+//   sums of x come from one more matrix instruction with ones, shared by the tile's 32 outputs.  16 is as small as the
+//   weights themselves, so the subtraction costs a few units of 2^-24 of the sum of the magnitudes.
+// * fp16: there is room for two nibbles below the exponent, 1024 + q and 1024 + 16 q, from which a subtraction or a fused
+//   multiply-add makes q - zero exactly: half as many shifts.
+// * The scale of a group multiplies its fp32 sum; nothing is rounded below 32 bits before the result is.
+// Infinities: (16 + q) * inf - (16 + zero) * inf is no number where (q - zero) * inf is one.  A warp whose sums are not
+// finite computes its stretch again with q - zero as the operand.
 //
-// A unit of work is 16 outputs of one expert; the warps of a block split its inputs (tiles warp, warp + 8, ...) and
-// their fp32 sums are added in warp order.  Only experts that have rows get units: every block lists them from the
-// offsets.
+// A unit of work is 32 outputs of one expert for up to eight of its rows; its tiles lie one behind the other in memory,
+// and so do the units of an expert.  Only experts that have rows get units: every block lists them from the offsets.  A
+// block gets a run of whole units, and its warps equal shares of the run's tiles, cut anywhere: a warp streams one
+// contiguous stretch of weights, kDepth tiles ahead of its products (cp.async into its own part of shared memory; it
+// waits for nothing but its own copies), writes the units that it has from end to end, and leaves the sums of the
+// cut ones (at most its first and its last) in shared memory, where after the block's only barrier the warp that began a
+// unit adds them in order.
 #include "row_types.cuh"
 
 namespace moe_rd {
@@ -24,98 +35,248 @@ int device_sms();
 
 namespace {
 
-constexpr int kW4Threads = 256;
+constexpr int kW4Threads = 512;
 constexpr int kW4Warps = kW4Threads / 32;
-constexpr int kW4BlocksPerSm = 2;
+constexpr int kDepth = 4;  // tiles in flight per warp
+constexpr int kTileBytes = 2048;
 
 struct W4Args {
   const unsigned char* x;
   const unsigned char* weight;
   const unsigned char* scales;
-  const uint8_t* zeros;
+  const unsigned char* zeros;
   const int32_t* offsets;
   unsigned char* out;
   int64_t rows;
-  int N, K, E, G, group;
-  int chunks;  // tiles of 128 inputs
-  int nblocks; // tiles of 16 outputs
+  int N, K, E, G;
+  int chunks;   // tiles of 128 inputs
+  int nblocks;  // blocks of 32 outputs
+  uint32_t group_magic;  // ceil(2^32 / (group / 32)): b / (group / 32) = (b * group_magic) >> 32 for b < 2^16; 0: group = 32
 };
+
+// SPAN: blocks of 32 inputs of a tile that share a group's scale: 4 (groups of a multiple of 128), 2 (64) or 1.
+template <int SPAN, bool ZEROS>
+struct W4Stage {
+  static constexpr int kParts = 4 / SPAN;                     // groups in a tile
+  static constexpr int kScales = kTileBytes;                  // [parts][8] four scales (outputs g, g + 8, g + 16, g + 24)
+  static constexpr int kZeros = kScales + 64 * kParts;        // [parts][8] their zero points, four bits each
+  static constexpr int kBytes = kZeros + (ZEROS ? 16 * kParts : 0);
+};
+
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
+  return r;
+}
+
+// A constant that the compiler keeps in a register (LOP3 takes one immediate, not two).
+template <uint32_t V>
+__device__ __forceinline__ uint32_t in_register() {
+  uint32_t r;
+  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "n"(V));
+  return r;
+}
 
 template <int DT>
 struct W4Type;
 
 template <>
 struct W4Type<MOE_RD_T_BF16> {
-  static constexpr uint32_t kBase = 0x43004300u;  // 128 in both halves; the last mantissa bit is worth 1
-  static constexpr int kOffset = 128;
-  static __device__ __forceinline__ float scale(const unsigned char* p, size_t i) {
-    return __uint_as_float((uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p) + i) << 16);
+  static constexpr bool kExact = false;  // operands are 16 + q
+  uint32_t mask = in_register<0x00780078u>(), base = in_register<0x41804180u>();
+  static __device__ __forceinline__ float first(uint32_t v) { return bf16_lo(v); }
+  static __device__ __forceinline__ float second(uint32_t v) { return bf16_hi(v); }
+  static __device__ __forceinline__ uint32_t zero_operand(uint32_t zero) { return 0x41804180u | (zero * 0x00080008u); }
+  __device__ __forceinline__ void unpack(uint32_t w, uint32_t, uint32_t (&o)[4]) const {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) o[p] = and_or(p ? __funnelshift_r(w, w, 4 * p) : w, mask, base);
   }
-  static __device__ __forceinline__ uint32_t both(int v) {
-    const __nv_bfloat162 b = __bfloat162bfloat162(__int2bfloat16_rn(v));
-    return *reinterpret_cast<const uint32_t*>(&b);
-  }
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
+  __device__ __forceinline__ void unpack_exact(uint32_t w, uint32_t zero, uint32_t (&o)[4]) const {
+    unpack(w, zero, o);
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&o[p]), *reinterpret_cast<const __nv_bfloat162*>(&zero));
+      o[p] = *reinterpret_cast<const uint32_t*>(&d);
+    }
   }
   static __device__ __forceinline__ uint16_t round(float v) {
     const __nv_bfloat16 b = __float2bfloat16_rn(v);
     return *reinterpret_cast<const uint16_t*>(&b);
   }
-  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
   }
+  static constexpr uint32_t kOnes = 0x3f803f80u;
 };
 
 template <>
 struct W4Type<MOE_RD_T_FP16> {
-  static constexpr uint32_t kBase = 0x64006400u;  // 1024 in both halves; the last mantissa bit is worth 1
-  static constexpr int kOffset = 1024;
-  static __device__ __forceinline__ float scale(const unsigned char* p, size_t i) {
-    return __half2float(__ushort_as_half(__ldg(reinterpret_cast<const uint16_t*>(p) + i)));
+  static constexpr bool kExact = true;  // operands are q - zero
+  uint32_t low = in_register<0x000f000fu>(), high = in_register<0x00f000f0u>(), base = in_register<0x64006400u>();
+  static __device__ __forceinline__ float first(uint32_t v) { return __low2float(*reinterpret_cast<const __half2*>(&v)); }
+  static __device__ __forceinline__ float second(uint32_t v) { return __high2float(*reinterpret_cast<const __half2*>(&v)); }
+  static __device__ __forceinline__ uint32_t zero_operand(uint32_t zero) { return 0x64006400u | (zero * 0x00010001u); }
+  __device__ __forceinline__ void unpack(uint32_t w, uint32_t zero, uint32_t (&o)[4]) const {
+    const uint32_t v = w >> 8;
+    // 1024 + zero -> -(64 + zero): the same bits of zero, sixteen times as high in the mantissa
+    const uint32_t z16 = ((zero & 0x000f000fu) << 4) | 0xd400d400u;
+    const uint32_t e[4] = {and_or(w, low, base), and_or(w, high, base), and_or(v, low, base), and_or(v, high, base)};
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const __half2 h = *reinterpret_cast<const __half2*>(&e[p]);
+      const __half2 d = p & 1 ? __hfma2(h, __float2half2_rn(0.0625f), *reinterpret_cast<const __half2*>(&z16))
+                              : __hsub2(h, *reinterpret_cast<const __half2*>(&zero));
+      o[p] = *reinterpret_cast<const uint32_t*>(&d);
+    }
   }
-  static __device__ __forceinline__ uint32_t both(int v) {
-    const __half2 b = __half2half2(__int2half_rn(v));
-    return *reinterpret_cast<const uint32_t*>(&b);
-  }
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
+  __device__ __forceinline__ void unpack_exact(uint32_t w, uint32_t zero, uint32_t (&o)[4]) const { unpack(w, zero, o); }
   static __device__ __forceinline__ uint16_t round(float v) { return __half_as_ushort(__float2half_rn(v)); }
-  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
   }
+  static constexpr uint32_t kOnes = 0x3c003c00u;
 };
 
-template <int DT>
-__device__ __forceinline__ uint32_t w4_pair(uint32_t word, int p, uint32_t zero) {
-  return W4Type<DT>::sub(((word >> (4 * p)) & 0x000f000fu) | W4Type<DT>::kBase, zero);
-}
-
-__device__ __forceinline__ uint4 ld_stream(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-
-template <int DT, bool ZEROS>
-__global__ void __launch_bounds__(kW4Threads, kW4BlocksPerSm) w4_kernel(const W4Args a) {
+// acc (+)= the product of one tile: w[2s + h] are the words of outputs 16s + 8h + g, x[q] the lane's inputs of block q,
+// scale(k, i) and zero(k, i) those of group k of the tile and output 8i + g.
+template <int DT, int SPAN, bool EXACT, typename Scale, typename Zero>
+__device__ __forceinline__ void w4_tile(const W4Type<DT>& ty, const uint4 (&w)[4], const uint4 (&x)[4], Scale scale, Zero zero,
+                                        float (&acc)[2][4]) {
   using Ty = W4Type<DT>;
+  const uint32_t word[4][4] = {{w[0].x, w[0].y, w[0].z, w[0].w}, {w[1].x, w[1].y, w[1].z, w[1].w},
+                               {w[2].x, w[2].y, w[2].z, w[2].w}, {w[3].x, w[3].y, w[3].z, w[3].w}};
+#pragma unroll
+  for (int k = 0; k < 4 / SPAN; ++k) {
+    float part[2][4], ones[4];
+#pragma unroll
+    for (int q = k * SPAN; q < (k + 1) * SPAN; ++q) {
+      const bool fresh = q == k * SPAN;
+      if (!EXACT) {
+        constexpr uint32_t one = Ty::kOnes;
+        if (fresh)
+          Ty::mma(ones, one, one, one, one, x[q].x, x[q].y, 0.0f, 0.0f, 0.0f, 0.0f);
+        else
+          Ty::mma(ones, one, one, one, one, x[q].x, x[q].y, ones[0], ones[1], ones[2], ones[3]);
+        Ty::mma(ones, one, one, one, one, x[q].z, x[q].w, ones[0], ones[1], ones[2], ones[3]);
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        uint32_t a[4], b[4];
+        if (EXACT) {
+          ty.unpack_exact(word[2 * s][q], zero(k, 2 * s), a);
+          ty.unpack_exact(word[2 * s + 1][q], zero(k, 2 * s + 1), b);
+        } else {
+          ty.unpack(word[2 * s][q], 0u, a);
+          ty.unpack(word[2 * s + 1][q], 0u, b);
+        }
+        if (fresh)
+          Ty::mma(part[s], a[0], b[0], a[1], b[1], x[q].x, x[q].y, 0.0f, 0.0f, 0.0f, 0.0f);
+        else
+          Ty::mma(part[s], a[0], b[0], a[1], b[1], x[q].x, x[q].y, part[s][0], part[s][1], part[s][2], part[s][3]);
+        Ty::mma(part[s], a[2], b[2], a[3], b[3], x[q].z, x[q].w, part[s][0], part[s][1], part[s][2], part[s][3]);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float p = part[s][i];
+        if (!EXACT) p = fmaf(-Ty::first(zero(k, 2 * s + (i >> 1))), ones[i & 1], p);
+        acc[s][i] = fmaf(scale(k, 2 * s + (i >> 1)), p, acc[s][i]);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+
+__device__ __forceinline__ uint32_t w4_group(const W4Args& a, uint32_t b) {  // of block b of 32 inputs
+  return min(a.group_magic != 0 ? __umulhi(b, a.group_magic) : b, (uint32_t)a.G - 1);
+}
+
+__device__ __forceinline__ void w4_load_x(const W4Args& a, const unsigned char* xp, int c, uint4 (&x)[4]) {
+  if (c < a.K >> 7) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = __ldg(reinterpret_cast<const uint4*>(xp + 64 * q));
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      x[q] = 128 * c + 32 * q < a.K ? __ldg(reinterpret_cast<const uint4*>(xp + 64 * q)) : make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+// Tiles [c0, c1) of a unit once more, with q - zero as the operand, straight from global memory.
+template <int DT, int SPAN, bool ZEROS>
+__device__ __noinline__ void w4_again(const W4Args& a, size_t block, int c0, int c1, const unsigned char* x_row, int lane,
+                                      float (&acc)[2][4]) {
+  const W4Type<DT> ty;
+  const int g = lane >> 2, j = lane & 3;
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[s][i] = 0.0f;
+  for (int c = c0; c < c1; ++c) {
+    uint4 w[4], x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = __ldg(reinterpret_cast<const uint4*>(a.weight + (block * a.chunks + c) * kTileBytes + i * 512 + lane * 16));
+    w4_load_x(a, x_row + (size_t)c * 256 + 16 * j, c, x);
+    w4_tile<DT, SPAN, true>(
+        ty, w, x,
+        [&](int k, int i) {
+          const size_t at = block * a.G + w4_group(a, 4 * c + SPAN * k);
+          const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(a.scales + at * 64 + g * 8) + (i >> 1));
+          return i & 1 ? W4Type<DT>::second(v) : W4Type<DT>::first(v);
+        },
+        [&](int k, int i) {
+          if (!ZEROS) return W4Type<DT>::zero_operand(8u);
+          const size_t at = block * a.G + w4_group(a, 4 * c + SPAN * k);
+          const uint32_t v = __ldg(reinterpret_cast<const uint16_t*>(a.zeros + at * 16) + g);
+          return W4Type<DT>::zero_operand((v >> (4 * i)) & 15u);
+        },
+        acc);
+  }
+}
+
+// n / d for 0 <= n < 2^62, d > 0
+__device__ __forceinline__ int64_t divide(int64_t n, int d) {
+  return (uint64_t)n >> 32 ? n / d : (int64_t)((uint32_t)n / (uint32_t)d);
+}
+
+// Where a warp is in its share of the block's tiles.
+struct W4Place {
+  int i, nb, pass;  // expert (of the list), block of 32 outputs, pass over eight rows
+  int c;            // tile of 128 inputs
+};
+
+template <int DT, int SPAN, bool ZEROS>
+__global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
+  using Ty = W4Type<DT>;
+  using St = W4Stage<SPAN, ZEROS>;
+  extern __shared__ __align__(16) unsigned char s_ring[];  // [warps][kDepth][St::kBytes]
   __shared__ int s_expert[kMaxE], s_lo[kMaxE], s_n[kMaxE], s_w[kW4Warps];
-  __shared__ float s_sum[kW4Warps][16 * 8];
+  __shared__ int64_t s_unit[kMaxE + 1], s_u[kW4Warps];
+  __shared__ float s_sum[kW4Warps][32 * 8];  // the end of a unit that another warp began
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, j = lane & 3;
+  const Ty ty;
   pdl_sync();
 
-  // experts that have rows, in order
+  // experts that have rows, in order, and the number of units before each
   int lo = 0, n = 0;
   int64_t first_row = 0, last_row = a.rows;
   if (a.offsets == nullptr) {
@@ -123,80 +284,213 @@ __global__ void __launch_bounds__(kW4Threads, kW4BlocksPerSm) w4_kernel(const W4
   } else {
     if (tid < a.E) {
       lo = max(__ldg(a.offsets + tid), 0);
-      n = min((int64_t)__ldg(a.offsets + tid + 1), a.rows) - lo;
+      n = (int)min((int64_t)__ldg(a.offsets + tid + 1), a.rows) - lo;
     }
     first_row = max(__ldg(a.offsets), 0);
     last_row = __ldg(a.offsets + a.E);
   }
-  const unsigned busy = __ballot_sync(kFull, n > 0);
-  if (lane == 0) s_w[warp] = __popc(busy);
-  __syncthreads();
-  int at = __popc(busy & ((1u << lane) - 1u)), experts = 0;
+  const int64_t mine = n > 0 ? (int64_t)((n + 7) >> 3) * a.nblocks : 0;
+  int64_t incl = mine;
 #pragma unroll
-  for (int w = 0; w < kW4Warps; ++w) {
-    if (w < warp) at += s_w[w];
-    experts += s_w[w];
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(kFull, incl, o);
+    if (lane >= o) incl += v;
+  }
+  const unsigned busy = __ballot_sync(kFull, n > 0);
+  if (lane == 31) {
+    s_w[warp] = __popc(busy);
+    s_u[warp] = incl;
+  }
+  __syncthreads();
+  int at = __popc(busy & ((1u << lane) - 1u));
+  int64_t units = 0, unit_at = incl - mine;
+#pragma unroll
+  for (int w = 0; w < kMaxE / 32; ++w) {
+    if (w < warp) {
+      at += s_w[w];
+      unit_at += s_u[w];
+    }
+    units += s_u[w];
   }
   if (n > 0) {
     s_expert[at] = tid;
     s_lo[at] = lo;
     s_n[at] = n;
+    s_unit[at] = unit_at;
+    s_unit[at + 1] = unit_at + mine;  // the next expert writes the same value
   }
   __syncthreads();
 
-  const int64_t units = (int64_t)experts * a.nblocks;
-  const int64_t u_end = units * (blockIdx.x + 1) / gridDim.x;
-  for (int64_t u = units * blockIdx.x / gridDim.x; u < u_end; ++u) {
-    const int i = (int)(u / a.nblocks), nb = (int)(u - (int64_t)i * a.nblocks);
-    const int e = s_expert[i], rows_e = s_n[i];
-    const size_t block = (size_t)e * a.nblocks + nb;
-    const unsigned char* wp = a.weight + block * a.chunks * 1024 + lane * 16;
-    const size_t sp = block * a.G * 16 + g;
-    for (int r0 = 0; r0 < rows_e; r0 += 8) {
-      const unsigned char* xp = a.x + ((size_t)(s_lo[i] + r0 + g) * a.K + 8 * j) * 2;
-      const bool has = r0 + g < rows_e;
-      float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int c = warp; c < a.chunks; c += kW4Warps) {
-        const uint4 wa = ld_stream(wp + (size_t)c * 1024), wb = ld_stream(wp + (size_t)c * 1024 + 512);
-        uint4 xv[4];
+  const int64_t u_first = divide(units * blockIdx.x, gridDim.x), u_end = divide(units * (blockIdx.x + 1), gridDim.x);
+  const int64_t tiles = (u_end - u_first) * a.chunks;
+  const int64_t t_first = tiles * warp / kW4Warps;
+  const int count = (int)(tiles * (warp + 1) / kW4Warps - t_first);
+  W4Place here = {0, 0, 0, 0};
+  if (count > 0) {
+    const int64_t ahead = divide(t_first, a.chunks), u = u_first + ahead;
+    here.c = (int)(t_first - ahead * a.chunks);
+    while (s_unit[here.i + 1] <= u) ++here.i;
+    const int passes = (s_n[here.i] + 7) >> 3;
+    const int64_t in = u - s_unit[here.i];
+    here.nb = (int)divide(in, passes);
+    here.pass = (int)(in - (int64_t)here.nb * passes);
+  }
+  // to the first tile of the next unit
+  auto next_unit = [&](W4Place& p) {
+    p.c = 0;
+    if (++p.pass * 8 < s_n[p.i]) return;
+    p.pass = 0;
+    if (++p.nb < a.nblocks) return;
+    p.nb = 0;
+    ++p.i;
+  };
+
+  // copies, kDepth tiles ahead
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_ring) + warp * kDepth * St::kBytes;
+  const unsigned char* ring_p = s_ring + warp * kDepth * St::kBytes;
+  W4Place next = here;
+  int to_fetch = count;
+  const unsigned char *next_w = nullptr, *next_s = nullptr, *next_z = nullptr;
+  auto aim = [&]() {
+    const size_t block = (size_t)s_expert[next.i] * a.nblocks + next.nb;
+    next_w = a.weight + (block * a.chunks + next.c) * kTileBytes + lane * 16;
+    next_s = a.scales + block * a.G * 64 + g * 8;
+    if (ZEROS) next_z = a.zeros + block * a.G * 16 + g * 4;
+  };
+  auto fetch = [&](int at_byte) {
+    if (to_fetch > 0) {
+      const uint32_t to = ring + at_byte;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          xv[q] = has && 128 * c + 32 * q < a.K ? __ldg(reinterpret_cast<const uint4*>(xp + (size_t)(128 * c + 32 * q) * 2))
-                                                : make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int gr = min((128 * c + 32 * q) / a.group, a.G - 1);
-          const float sa = Ty::scale(a.scales, sp + (size_t)gr * 16), sb = Ty::scale(a.scales, sp + (size_t)gr * 16 + 8);
-          const uint32_t za = Ty::both(Ty::kOffset + (ZEROS ? (int)__ldg(a.zeros + sp + (size_t)gr * 16) : 8));
-          const uint32_t zb = Ty::both(Ty::kOffset + (ZEROS ? (int)__ldg(a.zeros + sp + (size_t)gr * 16 + 8) : 8));
-          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          Ty::mma(part, w4_pair<DT>(ua[q], 0, za), w4_pair<DT>(ub[q], 0, zb), w4_pair<DT>(ua[q], 1, za),
-                  w4_pair<DT>(ub[q], 1, zb), xv[q].x, xv[q].y);
-          Ty::mma(part, w4_pair<DT>(ua[q], 2, za), w4_pair<DT>(ub[q], 2, zb), w4_pair<DT>(ua[q], 3, za),
-                  w4_pair<DT>(ub[q], 3, zb), xv[q].z, xv[q].w);
-          acc[0] = fmaf(sa, part[0], acc[0]);
-          acc[1] = fmaf(sa, part[1], acc[1]);
-          acc[2] = fmaf(sb, part[2], acc[2]);
-          acc[3] = fmaf(sb, part[3], acc[3]);
-        }
+      for (int i = 0; i < 4; ++i) copy16(to + i * 512 + lane * 16, next_w + i * 512);
+      if (j < St::kParts) {
+        const uint32_t gr = w4_group(a, 4 * next.c + SPAN * j);
+        copy8(to + St::kScales + (j * 8 + g) * 8, next_s + (size_t)gr * 64);
+        if (ZEROS && g < 4) copy4(to + St::kZeros + j * 16 + g * 4, next_z + (size_t)gr * 16);
       }
-      // [row of x][output]
-      s_sum[warp][(2 * j) * 16 + g] = acc[0];
-      s_sum[warp][(2 * j + 1) * 16 + g] = acc[1];
-      s_sum[warp][(2 * j) * 16 + g + 8] = acc[2];
-      s_sum[warp][(2 * j + 1) * 16 + g + 8] = acc[3];
-      __syncthreads();
-      if (tid < 128) {
-        float sum = s_sum[0][tid];
-#pragma unroll
-        for (int w = 1; w < kW4Warps; ++w) sum = __fadd_rn(sum, s_sum[w][tid]);
-        const int r = r0 + (tid >> 4), col = nb * 16 + (tid & 15);
-        if (r < rows_e && col < a.N)
-          reinterpret_cast<uint16_t*>(a.out)[(size_t)(s_lo[i] + r) * a.N + col] = Ty::round(sum);
+      next_w += kTileBytes;
+      if (++next.c == a.chunks && to_fetch > 1) {
+        next_unit(next);
+        aim();
       }
-      __syncthreads();
+      --to_fetch;
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (count > 0) aim();
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d) fetch(d * St::kBytes);
+
+  float acc[2][4];
+  const unsigned char* xp = nullptr;
+  bool began = here.c == 0;  // this warp has the unit from its first tile on
+  int c_first = here.c;      // the warp's first tile of the unit
+  auto begin = [&]() {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[s][i] = 0.0f;
+    // columns behind the unit's last row multiply that row again; their results are dropped
+    const int row = s_lo[here.i] + min(here.pass * 8 + g, s_n[here.i] - 1);
+    xp = a.x + ((size_t)row * a.K + here.c * 128 + 8 * j) * 2;
+    c_first = here.c;
+  };
+  // the sums of tiles [c_first, here.c) of the unit are complete
+  auto finish = [&]() {
+    if (!Ty::kExact) {
+      float probe = 0.0f;  // not finite if any of the sums is not
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) probe = fmaf(0.0f, acc[s][i], probe);
+      if (__any_sync(kFull, probe != 0.0f)) {
+        const size_t block = (size_t)s_expert[here.i] * a.nblocks + here.nb;
+        const int row = s_lo[here.i] + min(here.pass * 8 + g, s_n[here.i] - 1);
+        float again[2][4];  // its address leaves the function; acc's must not, or it would not stay in registers
+        w4_again<DT, SPAN, ZEROS>(a, block, c_first, here.c, a.x + (size_t)row * a.K * 2, lane, again);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[s][i] = again[s][i];
+      }
+    }
+  };
+  auto write = [&]() {
+    const int r0 = here.pass * 8, rows = s_n[here.i] - r0, cols = a.N - here.nb * 32 - g;
+    uint16_t* o = reinterpret_cast<uint16_t*>(a.out) + (size_t)(s_lo[here.i] + r0 + 2 * j) * a.N + here.nb * 32 + g;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (2 * j + (i & 1) < rows && 16 * s + 8 * (i >> 1) < cols) o[(size_t)(i & 1) * a.N + 16 * s + 8 * (i >> 1)] = Ty::round(acc[s][i]);
+  };
+  auto leave = [&]() {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s_sum[warp][(4 * s + i) * 32 + lane] = acc[s][i];
+  };
+
+  if (count > 0) begin();
+  int slot = 0;  // byte offset in the ring
+  for (int t = count; t > 0;) {
+    // the rest of this unit, or of the share
+    const int run = min(t, a.chunks - here.c);
+    t -= run;
+    for (const int c_end = here.c + run; here.c < c_end; ++here.c) {
+      uint4 x[4], w[4];
+      w4_load_x(a, xp, here.c, x);
+      xp += 256;
+      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+      __syncwarp();  // the scales of a tile are copied by all lanes
+      const unsigned char* st = ring_p + slot;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4*>(st + i * 512 + lane * 16);
+      uint2 sc[St::kParts];
+      uint32_t zp[St::kParts];
+#pragma unroll
+      for (int k = 0; k < St::kParts; ++k) {
+        sc[k] = *reinterpret_cast<const uint2*>(st + St::kScales + (k * 8 + g) * 8);
+        zp[k] = ZEROS ? *reinterpret_cast<const uint16_t*>(st + St::kZeros + k * 16 + g * 2) : 0x8888u;
+      }
+      __syncwarp();
+      fetch(slot);
+      slot = slot + St::kBytes == kDepth * St::kBytes ? 0 : slot + St::kBytes;
+      w4_tile<DT, SPAN, Ty::kExact>(
+          ty, w, x,
+          [&](int k, int i) {
+            const uint32_t v = i < 2 ? sc[k].x : sc[k].y;
+            return i & 1 ? Ty::second(v) : Ty::first(v);
+          },
+          [&](int k, int i) { return Ty::zero_operand((zp[k] >> (4 * i)) & 15u); }, acc);
+    }
+    finish();
+    if (t > 0) {
+      if (began)
+        write();
+      else
+        leave();
+      next_unit(here);
+      began = true;
+      begin();
+    }
+  }
+  // the last unit: finished or not, begun here or not
+  if (count > 0 && !began) leave();
+  __syncthreads();
+  if (count > 0 && began) {
+    int64_t end = t_first + count;                          // tiles of the run that are in acc
+    const int64_t unit_end = end + (a.chunks - here.c);
+    for (int w = warp + 1; end < unit_end; ++w) {            // the warps that have the rest of the unit
+      const int64_t w_end = tiles * (w + 1) / kW4Warps;
+      if (w_end > end) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[s][i] = __fadd_rn(acc[s][i], s_sum[w][(4 * s + i) * 32 + lane]);
+        end = w_end;
+      }
+    }
+    write();
   }
 
   // rows of no expert
@@ -208,48 +502,65 @@ __global__ void __launch_bounds__(kW4Threads, kW4BlocksPerSm) w4_kernel(const W4
     reinterpret_cast<uint16_t*>(a.out)[k < before ? k : last_row * a.N + (k - before)] = 0;
 }
 
+template <int DT, int SPAN, bool ZEROS>
+cudaError_t launch_w4(const W4Args& a, cudaStream_t s) {
+  constexpr int smem = kW4Warps * kDepth * W4Stage<SPAN, ZEROS>::kBytes;
+  // per device, and cheap: the attribute is set before every launch, so no state is kept
+  const cudaError_t e = cudaFuncSetAttribute(w4_kernel<DT, SPAN, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(w4_kernel<DT, SPAN, ZEROS>, dim3((unsigned)device_sms()), dim3(kW4Threads), smem, s, a);
+}
+
+template <int DT, bool ZEROS>
+cudaError_t launch_w4_span(const W4Args& a, int group, cudaStream_t s) {
+  if (group % 128 == 0) return launch_w4<DT, 4, ZEROS>(a, s);
+  if (group % 64 == 0) return launch_w4<DT, 2, ZEROS>(a, s);
+  return launch_w4<DT, 1, ZEROS>(a, s);
+}
+
 }  // namespace
 }  // namespace moe_rd
 
 using namespace moe_rd;
 
 extern "C" int moe_rd_expert_matvec_w4(int64_t rows, int32_t N, int32_t K, int32_t E, int32_t group, int32_t dtype,
-                                       const void* x, const void* weight, const void* scales, const uint8_t* zeros,
+                                       const void* x, const void* weight, const void* scales, const uint16_t* zeros,
                                        const int32_t* offsets, void* out, void* stream) {
   if (dtype == MOE_RD_T_F32) return MOE_RD_E_UNSUPPORTED;
   if (dtype != MOE_RD_T_BF16 && dtype != MOE_RD_T_FP16) return MOE_RD_E_ENUM;
-  if (rows < 0 || rows > 0x7fffffff || N < 1 || N > (1 << 24) || K < 32 || K > (1 << 20) || E < 1 || E > kMaxE ||
+  if (rows < 0 || rows > (1 << 30) || N < 1 || N > (1 << 24) || K < 32 || K > (1 << 20) || E < 1 || E > kMaxE ||
       group < 32 || group % 32 != 0 || K % group != 0 || (offsets == nullptr && E != 1))
     return MOE_RD_E_SHAPE;
+  // a warp counts its tiles in 32 bits
+  if ((rows / 8 + E) * ((N + 31) / 32) > ((int64_t)1 << 40) / ((K + 127) / 128)) return MOE_RD_E_TOO_LARGE;
   if (rows == 0) return MOE_RD_OK;
   if (x == nullptr || weight == nullptr || scales == nullptr || out == nullptr) return MOE_RD_E_NULL;
-  if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(weight)) & 15 ||
-      (reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(scales)) & 1)
+  if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(scales) |
+       reinterpret_cast<uintptr_t>(zeros)) & 15 ||
+      reinterpret_cast<uintptr_t>(out) & 1)
     return MOE_RD_E_ALIGN;
   W4Args a = {};
   a.x = static_cast<const unsigned char*>(x);
   a.weight = static_cast<const unsigned char*>(weight);
   a.scales = static_cast<const unsigned char*>(scales);
-  a.zeros = zeros;
+  a.zeros = reinterpret_cast<const unsigned char*>(zeros);
   a.offsets = offsets;
   a.out = static_cast<unsigned char*>(out);
   a.rows = rows;
   a.N = N;
   a.K = K;
   a.E = E;
-  a.group = group;
   a.G = K / group;
   a.chunks = (K + 127) / 128;
-  a.nblocks = (N + 15) / 16;
-  const dim3 grid((unsigned)(device_sms() * kW4BlocksPerSm));
+  a.nblocks = (N + 31) / 32;
+  const uint32_t per = (uint32_t)group / 32;
+  a.group_magic = per == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + per - 1) / per);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (dtype == MOE_RD_T_BF16)
-    e = zeros != nullptr ? launch_pdl(w4_kernel<MOE_RD_T_BF16, true>, grid, dim3(kW4Threads), 0, s, a)
-                         : launch_pdl(w4_kernel<MOE_RD_T_BF16, false>, grid, dim3(kW4Threads), 0, s, a);
+    e = zeros != nullptr ? launch_w4_span<MOE_RD_T_BF16, true>(a, group, s) : launch_w4_span<MOE_RD_T_BF16, false>(a, group, s);
   else
-    e = zeros != nullptr ? launch_pdl(w4_kernel<MOE_RD_T_FP16, true>, grid, dim3(kW4Threads), 0, s, a)
-                         : launch_pdl(w4_kernel<MOE_RD_T_FP16, false>, grid, dim3(kW4Threads), 0, s, a);
+    e = zeros != nullptr ? launch_w4_span<MOE_RD_T_FP16, true>(a, group, s) : launch_w4_span<MOE_RD_T_FP16, false>(a, group, s);
   count_launch();
   if (e != cudaSuccess) {
     set_last_cuda_error(e);

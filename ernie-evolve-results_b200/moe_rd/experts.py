@@ -13,20 +13,21 @@ from .sorting import _aligned, _check_offsets, _ptr, call, check_device, check_o
 
 class W4Weights(NamedTuple):
     """4-bit weights in the layout of the kernel (see ``moe_rd_expert_matvec_w4`` in include/moe_rd.h)."""
-    packed: torch.Tensor           # [E, ceil(N/16), ceil(K/128), 1024] uint8
-    scales: torch.Tensor           # [E, ceil(N/16), K/group, 16] bf16 or fp16
-    zeros: Optional[torch.Tensor]  # the same shape, uint8; None: every zero point is 8
+    packed: torch.Tensor           # [E, ceil(N/32), ceil(K/128), 2048] uint8
+    scales: torch.Tensor           # [E, ceil(N/32), K/group, 8, 4] bf16 or fp16
+    zeros: Optional[torch.Tensor]  # [E, ceil(N/32), K/group, 8, 2] uint8, two zero points a byte; None: all are 8
     N: int
     K: int
     group: int
 
 
 def _blocked(t: torch.Tensor) -> torch.Tensor:
-    """[E, N, G] per-group values as [E, ceil(N/16), G, 16], zero-padded."""
+    """[E, N, G] per-group values as [E, ceil(N/32), G, 8, 4], zero-padded; outputs r, r + 8, r + 16, r + 24 of a block side
+    by side."""
     E, N, G = t.shape
-    full = t.new_zeros((E, -(-N // 16) * 16, G))
+    full = t.new_zeros((E, -(-N // 32) * 32, G))
     full[:, :N] = t
-    return full.reshape(E, -1, 16, G).transpose(2, 3).contiguous()
+    return full.reshape(E, -1, 4, 8, G).permute(0, 1, 4, 3, 2).contiguous()
 
 
 def pack_w4(q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None) -> W4Weights:
@@ -58,17 +59,22 @@ def pack_w4(q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor]
     for t in (scales, zeros):
         if t is not None and t.device != q.device:
             raise ValueError("pack_w4: all tensors must be on one device")
-    blocks, chunks = -(-N // 16), -(-K // 128)
-    full = q.new_zeros((E, blocks * 16, chunks * 64))
+    blocks, chunks = -(-N // 32), -(-K // 128)
+    full = q.new_zeros((E, blocks * 32, chunks * 64))
     full[:, :N, :half] = q
-    # [E, block, half, output, chunk, word i, lane j, byte] -> [E, block, chunk, half, output, j, i, byte]
-    r = full.reshape(E, blocks, 2, 8, chunks, 4, 4, 4).permute(0, 1, 4, 2, 3, 6, 5, 7)
+    # [E, block, part, output, chunk, word, lane j, byte] -> [E, block, chunk, part, output, j, word, byte]
+    r = full.reshape(E, blocks, 4, 8, chunks, 4, 4, 4).permute(0, 1, 4, 2, 3, 6, 5, 7)
     packed = torch.empty(r.shape, dtype=torch.uint8, device=q.device)
     packed[..., 0] = (r[..., 0] & 15) | ((r[..., 1] & 15) << 4)
     packed[..., 1] = (r[..., 2] & 15) | ((r[..., 3] & 15) << 4)
     packed[..., 2] = (r[..., 0] >> 4) | (r[..., 1] & 0xF0)
     packed[..., 3] = (r[..., 2] >> 4) | (r[..., 3] & 0xF0)
-    return W4Weights(packed.reshape(E, blocks, chunks, 1024), _blocked(scales), None if zeros is None else _blocked(zeros), N, K, group)
+    if scales.dtype == torch.bfloat16:  # rotate every word left by three bits
+        packed = (packed << 3) | (packed.roll(1, -1) >> 5)
+    if zeros is not None:
+        z = _blocked(zeros)
+        zeros = z[..., 0::2] | (z[..., 1::2] << 4)
+    return W4Weights(packed.reshape(E, blocks, chunks, 2048), _blocked(scales), zeros, N, K, group)
 
 
 def expert_matvec_w4(x: torch.Tensor, weights: W4Weights, offsets: Optional[torch.Tensor] = None, *,
@@ -93,9 +99,9 @@ def expert_matvec_w4(x: torch.Tensor, weights: W4Weights, offsets: Optional[torc
     G = K // weights.group
     if x.dim() != 2 or x.shape[1] != K:
         raise ValueError(f"expert_matvec_w4: rows must be [R, {K}]")
-    if (weights.packed.shape != (E, -(-N // 16), -(-K // 128), 1024) or weights.packed.dtype != torch.uint8
-            or weights.scales.shape != (E, blocks, G, 16) or not weights.packed.is_contiguous() or not weights.scales.is_contiguous()
-            or (weights.zeros is not None and (weights.zeros.shape != weights.scales.shape or weights.zeros.dtype != torch.uint8
+    if (weights.packed.shape != (E, -(-N // 32), -(-K // 128), 2048) or weights.packed.dtype != torch.uint8
+            or weights.scales.shape != (E, blocks, G, 8, 4) or not weights.packed.is_contiguous() or not weights.scales.is_contiguous()
+            or (weights.zeros is not None and (weights.zeros.shape != (E, blocks, G, 8, 2) or weights.zeros.dtype != torch.uint8
                                                or not weights.zeros.is_contiguous()))):
         raise ValueError("expert_matvec_w4: weights are not as pack_w4 returns them")
     _check_offsets("expert_matvec_w4", offsets)

@@ -479,16 +479,19 @@ int moe_rd_routing_weights_backward(int64_t T, int32_t E, int32_t K, int32_t sco
  * scaled in fp32; the result is rounded once.  Every weight of an expert that has
  * rows is read once per eight of its rows, so the call is meant for few rows per
  * expert; it is right for any number.
- * K % group == 0, group % 32 == 0; x and out 16-byte aligned.  The weights are laid
- * out in tiles of 16 outputs x 128 inputs (with C = ceil(K/128), B = ceil(N/16),
- * G = K/group), zero-padded:
- *   weight [E][B][C][1024 bytes]: half h (outputs 16b + 8h + 0..7), lane l = 4*r + j
- *     (r: output inside the half), word i (16 bytes a lane): the eight inputs
- *     128c + 32i + 8j + 0..7 of that output; input 2p in bits 4p.., input 2p+1 in bits 16+4p..
- *   scales [E][B][G][16], zeros [E][B][G][16] (one byte each)
+ * K % group == 0, group % 32 == 0, K <= 2^20, rows <= 2^30; x, weight, scales and
+ * zeros 16-byte aligned.  The weights are laid
+ * out in tiles of 32 outputs x 128 inputs, zero-padded (C = ceil(K/128), B =
+ * ceil(N/32), G = K/group):
+ *   weight [E][B][C][4][32][4] 32-bit words: part i (outputs 32b + 8i + 0..7), lane
+ *     4*r + j (output r of the part), word m: the eight inputs 128c + 32m + 8j +
+ *     0..7 of that output, input 2p in bits 4p.. and input 2p+1 in bits 16+4p..;
+ *     for bf16 the whole word rotated left by three bits
+ *   scales [E][B][G][8][4] (outputs r, r + 8, r + 16, r + 24 of the block)
+ *   zeros  [E][B][G][8]    16 bits: four bits for each of the same outputs, lowest first
  */
 int moe_rd_expert_matvec_w4(int64_t rows, int32_t N, int32_t K, int32_t E, int32_t group, int32_t dtype,
-                            const void* x, const void* weight, const void* scales, const uint8_t* zeros,
+                            const void* x, const void* weight, const void* scales, const uint16_t* zeros,
                             const int32_t* offsets, void* out, void* stream);
 
 /* Kernels this library launched since it was loaded (all threads). */

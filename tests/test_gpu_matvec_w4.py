@@ -21,19 +21,26 @@ def make(E, N, K, group, dtype, zeros, seed=0):
     return q, s, z, w
 
 
-def check(x, w, offsets, got, dtype, K):
+def check(x, w, s, offsets, got, dtype, K):
     want = torch.zeros(got.shape, dtype=torch.float64)
     mag = torch.zeros_like(want)
     for e in range(w.shape[0]):
         lo, hi = offsets[e], offsets[e + 1]
         want[lo:hi] = x[lo:hi].double() @ w[e].t()
         mag[lo:hi] = x[lo:hi].double().abs() @ w[e].t().abs()
-    # the products are exact; a matrix instruction adds 16 of them to its sum, each addend within 2 units of 2^-24 of the
-    # largest: 34; two to a group's part, one product and one addition per 32 inputs of a warp's share, 8 warps
-    low = (2 * 34 + 2 * (K / 32) + 8) * 2.0 ** -24 * mag
+    # a matrix instruction adds 16 exact products to its sum, each addend within a unit of 2^-24 of the largest: 17; eight to
+    # a group's part; operands of at most 31 for the part (16 + q) and for what is taken off it (16 + zero); then one
+    # product and one addition per 32 inputs of the row, and 16 warps
+    size = torch.zeros_like(want)
+    for e in range(w.shape[0]):
+        lo, hi = offsets[e], offsets[e + 1]
+        size[lo:hi] = x[lo:hi].double().abs() @ s[e].double().repeat_interleave(K // s.shape[2], 1).t()
+    low = 2 * 8 * 17 * 2.0 ** -24 * 31 * size + (2 * (K / 32) + 16) * 2.0 ** -24 * mag
     bound = low + HALF_STEP[dtype] * (want.abs() + low) + TINY[dtype]
     err = (got.cpu().double() - want).abs()
     assert (err <= bound).all(), float((err / bound).max())
+    # the roundings to the result's type alone may be half a step everywhere; they average 0.58 of that
+    assert err.norm() <= HALF_STEP[dtype] * want.norm() + TINY[dtype] * err.numel()
 
 
 CASES = [
@@ -64,7 +71,7 @@ def test_expert_products(E, N, K, group, dtype, zeros, rows, behind):
     packed = moe_rd.pack_w4(q.cuda(), s.cuda(), None if z is None else z.cuda())
     off = torch.tensor(offsets, dtype=torch.int32).cuda()
     got = moe_rd.expert_matvec_w4(x.cuda(), packed, off)
-    check(x, w, offsets, got, dtype, K)
+    check(x, w, s, offsets, got, dtype, K)
     assert (got[offsets[-1]:] == 0).all()
     buf = torch.full_like(got, float("nan"))
     assert moe_rd.expert_matvec_w4(x.cuda(), packed, off, out=buf) is buf and torch.equal(buf, got)
@@ -83,16 +90,26 @@ def test_every_value_and_zero_point_is_exact():
         assert torch.equal(got.float().cpu(), ((value - z.float()) * 0.25).t())
 
 
-def test_nan_and_inf_reach_only_their_rows_and_outputs():
-    q, s, z, w = make(1, 40, 256, 64, "bf16", True)
-    x = torch.randn(5, 256).to(torch.bfloat16)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_nan_and_inf_reach_only_their_rows_and_outputs(dtype):
+    """An infinity in a row gives what the formula gives: an infinity of the weight's sign, or no number where the weight is
+    zero; rows next to it, and values near the end of the range, are as exact as ever."""
+    q, s, z, w = make(1, 40, 1152, 64, dtype, True)
+    s[0, 7, 1] = float("nan")
+    w[0, 7] = float("nan")
+    x = torch.randn(7, 1152).to(DT[dtype])
     x[2, 9] = float("inf")
     x[3, 200] = float("nan")
-    s[0, 7, 1] = float("nan")
+    x[5, 1100] = -float("inf")
+    x[6] = torch.finfo(DT[dtype]).max / 4096      # sixteen times a sum of these has no place in the range
     got = moe_rd.expert_matvec_w4(x.cuda(), moe_rd.pack_w4(q.cuda(), s.cuda(), z.cuda())).cpu()
     keep = torch.arange(40) != 7
-    assert torch.isfinite(got[[0, 1, 4]][:, keep]).all() and torch.isnan(got[:, 7]).all()
-    assert torch.isnan(got[3]).all() and not torch.isfinite(got[2, keep]).any()
+    assert torch.isnan(got[:, 7]).all() and torch.isnan(got[3]).all()
+    for r, k, sign in ((2, 9, 1.0), (5, 1100, -1.0)):
+        inf = torch.full((40,), float("inf"), dtype=torch.float64) * sign * w[0, :, k]
+        assert torch.equal(torch.nan_to_num(got[r, keep].double(), nan=7.0), torch.nan_to_num(inf[keep], nan=7.0))
+    rows = [0, 1, 4, 6]
+    check(x[rows], w[:, keep], s[:, keep], [0, 4], got[rows][:, keep], dtype, 1152)
 
 
 def test_the_decode_step_of_a_layer():

@@ -65,23 +65,29 @@ def test_routing_weight_refusals():
         moe_rd.routing_weights_backward(x(4, 2, dtype=torch.float32), lg, ids)
 
 
-def test_pack_w4_layout_and_refusals():
-    E, N, K, group = 2, 21, 160, 32
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_pack_w4_layout_and_refusals(dtype):
+    E, N, K, group = 2, 45, 160, 32
     g = torch.Generator().manual_seed(1)
     q = torch.randint(0, 256, (E, N, K // 2), generator=g, dtype=torch.uint8)
-    s = torch.rand(E, N, K // group, generator=g).to(torch.bfloat16)
+    s = torch.rand(E, N, K // group, generator=g).to(dtype)
     z = torch.randint(0, 16, s.shape, generator=g, dtype=torch.uint8)
     p = moe_rd.pack_w4(q, s, z)
-    assert (p.N, p.K, p.group) == (N, K, group) and p.packed.shape == (E, 2, 2, 1024) and p.scales.shape == (E, 2, 5, 16)
+    assert (p.N, p.K, p.group) == (N, K, group) and p.packed.shape == (E, 2, 2, 2048) and p.scales.shape == (E, 2, 5, 8, 4)
     value = torch.stack([q & 15, q >> 4], -1).reshape(E, N, K)
-    for e, n, k in [(0, 0, 0), (0, 0, 1), (1, 20, 159), (0, 7, 31), (1, 8, 32), (0, 15, 127), (1, 16, 128), (0, 13, 77)]:
-        b, c, h, r = n // 16, k // 128, (n % 16) // 8, n % 8
-        i, j, kk = (k % 128) // 32, (k % 32) // 8, k % 8
-        at = h * 512 + (4 * r + j) * 16 + 4 * i
+    for e, n, k in [(0, 0, 0), (0, 0, 1), (1, 44, 159), (0, 7, 31), (1, 8, 32), (0, 15, 127), (1, 16, 128), (0, 29, 77), (0, 43, 6)]:
+        b, c, part, r = n // 32, k // 128, (n % 32) // 8, n % 8
+        m, j, kk = (k % 128) // 32, (k % 32) // 8, k % 8
+        at = part * 512 + (4 * r + j) * 16 + 4 * m
         word = int.from_bytes(bytes(p.packed[e, b, c, at:at + 4].tolist()), "little")
+        if dtype == torch.bfloat16:
+            word = (word >> 3) | ((word & 7) << 29)
         assert (word >> (4 * (kk // 2) + 16 * (kk % 2))) & 15 == int(value[e, n, k])
-        assert p.scales[e, b, k // group, n % 16] == s[e, n, k // group] and p.zeros[e, b, k // group, n % 16] == z[e, n, k // group]
-    assert (p.scales[:, 1, :, 5:] == 0).all() and int(p.packed[:, 1, :, 512:].sum()) == 0     # outputs past N
+        assert p.scales[e, b, k // group, r, part] == s[e, n, k // group]
+        word = int.from_bytes(bytes(p.zeros[e, b, k // group, r].tolist()), "little")
+        assert (word >> (4 * part)) & 15 == int(z[e, n, k // group])
+    assert (p.scales[:, 1, :, 5:, 1] == 0).all() and (p.scales[:, 1, :, :, 2:] == 0).all()     # outputs past N
+    assert int(p.packed[:, 1, :, 1024:].sum()) == 0
     one = moe_rd.pack_w4(q[0], s[0], z[0])
     assert all(torch.equal(a, b[:1]) for a, b in zip(one[:3], p[:3]))
     for args, why in (((q.int(), s), TypeError), ((q, s.float()), TypeError), ((q, s[:, :20]), ValueError), ((q, s[..., :3]), ValueError),
@@ -89,9 +95,9 @@ def test_pack_w4_layout_and_refusals():
                       ((q[..., :8], s[..., :1]), ValueError)):
         with pytest.raises(why):
             moe_rd.pack_w4(*args)
-    rows = x(3, K)
+    rows = x(3, K, dtype=dtype)
     off = torch.tensor([0, 1, 3], dtype=I32)
-    for args, why in (((rows, q), TypeError), ((rows.float(), p, off), TypeError), ((rows.half(), p, off), TypeError),
+    for args, why in (((rows, q), TypeError), ((rows.float(), p, off), TypeError), ((rows.to(torch.float16 if dtype == torch.bfloat16 else torch.bfloat16), p, off), TypeError),
                       ((rows[:, :128], p, off), ValueError), ((rows, p), ValueError), ((rows, p, off[:2]), ValueError),
                       ((rows, p, off.long()), TypeError), ((rows.requires_grad_(), p, off), RuntimeError),
                       ((rows.detach(), p._replace(packed=p.packed[:, :1]), off), ValueError), ((rows.detach(), p, off), RuntimeError)):
