@@ -25,8 +25,9 @@
 // block gets a run of whole units, and its warps equal shares of the run's tiles, cut anywhere: a warp streams one
 // contiguous stretch of weights, kDepth tiles ahead of its products (cp.async into its own part of shared memory; it
 // waits for nothing but its own copies), writes the units that it has from end to end, and leaves the sums of the
-// cut ones (at most its first and its last) in shared memory, where after the block's only barrier the warp that began a
-// unit adds them in order.
+// cut ones (at most its first and its last) in shared memory, where after a barrier they are added in the warps' order.
+#include <limits.h>
+
 #include "row_types.cuh"
 
 namespace moe_rd {
@@ -252,48 +253,77 @@ __device__ __noinline__ void w4_again(const W4Args& a, size_t block, int c0, int
   }
 }
 
-// n / d for 0 <= n < 2^62, d > 0
-__device__ __forceinline__ int64_t divide(int64_t n, int d) {
-  return (uint64_t)n >> 32 ? n / d : (int64_t)((uint32_t)n / (uint32_t)d);
-}
-
 // Where a warp is in its share of the block's tiles.
 struct W4Place {
   int i, nb, pass;  // expert (of the list), block of 32 outputs, pass over eight rows
   int c;            // tile of 128 inputs
 };
 
+// What a warp has left in shared memory: the part of a unit that an earlier warp began, with or without its end, and the
+// part of a unit that it began itself and later warps end.
+enum { kContinues = 1, kEnds = 2, kBegins = 4 };
+
+struct W4Joint {
+  float sum[2 * kW4Warps][32 * 8];  // [warp]: the part of the first unit; [kW4Warps + warp]: of the last; [row of x][output]
+  W4Place place[kW4Warps];          // of the unit that the warp began
+  int what[kW4Warps];
+  int expert[kMaxE], lo[kMaxE], n[kMaxE], unit[kMaxE];  // experts that have rows: number, rows, units before
+};
+
+// The units that several warps have: a thread per sum, 256 a unit, added in the order of the warps.  Called once with
+// rows = 0, which writes nothing, while the first tiles are on their way: the instructions would otherwise have to be
+// fetched through a memory system that is busy with weights, 2 us at the end of every call.
+template <int DT>
+__device__ __noinline__ void w4_join(const W4Args& a, const W4Joint& s, int rows) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int what = lane < kW4Warps ? s.what[lane] : 0;
+  const unsigned continues = __ballot_sync(kFull, what & kContinues), ends = __ballot_sync(kFull, what & kEnds);
+  unsigned begins = __ballot_sync(kFull, what & kBegins);
+  for (int k = 0; begins != 0; ++k, begins &= begins - 1) {
+    if ((k & 1) != tid >> 8) continue;
+    const int w = __ffs(begins) - 1;
+    const int last = w + __ffs(ends >> (w + 1));
+    const W4Place p = s.place[w];
+    const int el = tid & 255, r = p.pass * 8 + (el >> 5), col = p.nb * 32 + (el & 31);
+    float sum = s.sum[kW4Warps + w][el];
+#pragma unroll
+    for (int v = 1; v < kW4Warps; ++v)
+      if (v > w && v <= last && ((continues >> v) & 1u)) sum = __fadd_rn(sum, s.sum[v][el]);
+    if (r < min(rows, s.n[p.i]) && col < a.N) reinterpret_cast<uint16_t*>(a.out)[(size_t)(s.lo[p.i] + r) * a.N + col] = W4Type<DT>::round(sum);
+  }
+}
+
 template <int DT, int SPAN, bool ZEROS>
 __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
   using Ty = W4Type<DT>;
   using St = W4Stage<SPAN, ZEROS>;
   extern __shared__ __align__(16) unsigned char s_ring[];  // [warps][kDepth][St::kBytes]
-  __shared__ int s_expert[kMaxE], s_lo[kMaxE], s_n[kMaxE], s_w[kW4Warps];
-  __shared__ int64_t s_unit[kMaxE + 1], s_u[kW4Warps];
-  __shared__ float s_sum[kW4Warps][32 * 8];  // the end of a unit that another warp began
+  __shared__ int s_w[kW4Warps], s_u[kW4Warps];
+  __shared__ W4Joint s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, j = lane & 3;
   const Ty ty;
   pdl_sync();
 
-  // experts that have rows, in order, and the number of units before each
-  int lo = 0, n = 0;
-  int64_t first_row = 0, last_row = a.rows;
+  // experts that have rows, in order, and the number of units before each (all counts are below 2^31, see the entry)
+  int lo = 0, n = 0, first_row = 0, last_row = (int)a.rows;
   if (a.offsets == nullptr) {
     n = tid == 0 ? (int)a.rows : 0;
   } else {
     if (tid < a.E) {
-      lo = max(__ldg(a.offsets + tid), 0);
-      n = (int)min((int64_t)__ldg(a.offsets + tid + 1), a.rows) - lo;
+      lo = __ldg(a.offsets + tid);
+      n = __ldg(a.offsets + tid + 1) - lo;
+      // offsets that decrease or leave the rows are nobody's: every row becomes zero
+      if (lo < 0 || n < 0 || n > (int)a.rows - lo) n = INT_MIN;
     }
-    first_row = max(__ldg(a.offsets), 0);
+    first_row = __ldg(a.offsets);
     last_row = __ldg(a.offsets + a.E);
   }
-  const int64_t mine = n > 0 ? (int64_t)((n + 7) >> 3) * a.nblocks : 0;
-  int64_t incl = mine;
+  const int mine = n > 0 ? ((n + 7) >> 3) * a.nblocks : 0;
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(kFull, incl, o);
+    const int v = __shfl_up_sync(kFull, incl, o);
     if (lane >= o) incl += v;
   }
   const unsigned busy = __ballot_sync(kFull, n > 0);
@@ -301,44 +331,57 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
     s_w[warp] = __popc(busy);
     s_u[warp] = incl;
   }
-  __syncthreads();
-  int at = __popc(busy & ((1u << lane) - 1u));
-  int64_t units = 0, unit_at = incl - mine;
+  const bool broken = __syncthreads_or(n == INT_MIN);
+  int at = __popc(busy & ((1u << lane) - 1u)), experts = 0, units = 0, unit_at = incl - mine;
 #pragma unroll
   for (int w = 0; w < kMaxE / 32; ++w) {
     if (w < warp) {
       at += s_w[w];
       unit_at += s_u[w];
     }
+    experts += s_w[w];
     units += s_u[w];
   }
   if (n > 0) {
-    s_expert[at] = tid;
-    s_lo[at] = lo;
-    s_n[at] = n;
-    s_unit[at] = unit_at;
-    s_unit[at + 1] = unit_at + mine;  // the next expert writes the same value
+    s.expert[at] = tid;
+    s.lo[at] = lo;
+    s.n[at] = n;
+    s.unit[at] = unit_at;
+  }
+  if (broken) {
+    units = 0;
+    first_row = last_row = 0;
+  }
+  if (tid < kW4Warps) {  // for the call of w4_join that writes nothing
+    s.what[tid] = tid < 2 ? kBegins : kContinues | kEnds;
+    s.place[tid] = W4Place{0, 0, 0, 0};
   }
   __syncthreads();
 
-  const int64_t u_first = divide(units * blockIdx.x, gridDim.x), u_end = divide(units * (blockIdx.x + 1), gridDim.x);
-  const int64_t tiles = (u_end - u_first) * a.chunks;
-  const int64_t t_first = tiles * warp / kW4Warps;
-  const int count = (int)(tiles * (warp + 1) / kW4Warps - t_first);
+  const int even = units / gridDim.x, odd = units - even * gridDim.x;  // the first `odd` blocks have one unit more
+  const int u_first = even * blockIdx.x + min((int)blockIdx.x, odd);
+  const int tiles = (even + ((int)blockIdx.x < odd ? 1 : 0)) * a.chunks;
+  const int t_first = (int)((int64_t)tiles * warp / kW4Warps);
+  const int count = (int)((int64_t)tiles * (warp + 1) / kW4Warps) - t_first;
   W4Place here = {0, 0, 0, 0};
   if (count > 0) {
-    const int64_t ahead = divide(t_first, a.chunks), u = u_first + ahead;
-    here.c = (int)(t_first - ahead * a.chunks);
-    while (s_unit[here.i + 1] <= u) ++here.i;
-    const int passes = (s_n[here.i] + 7) >> 3;
-    const int64_t in = u - s_unit[here.i];
-    here.nb = (int)divide(in, passes);
-    here.pass = (int)(in - (int64_t)here.nb * passes);
+    const int ahead = t_first / a.chunks, u = u_first + ahead;
+    here.c = t_first - ahead * a.chunks;
+    // the last expert whose first unit is not behind u
+    for (int i0 = 0;; i0 += 32) {
+      const unsigned m = __ballot_sync(kFull, i0 + lane < experts && s.unit[i0 + lane] <= u);
+      here.i += __popc(m);
+      if (m != kFull) break;
+    }
+    --here.i;
+    const int in = u - s.unit[here.i], passes = (s.n[here.i] + 7) >> 3;
+    here.nb = passes == 1 ? in : in / passes;
+    here.pass = in - here.nb * passes;
   }
   // to the first tile of the next unit
   auto next_unit = [&](W4Place& p) {
     p.c = 0;
-    if (++p.pass * 8 < s_n[p.i]) return;
+    if (++p.pass * 8 < s.n[p.i]) return;
     p.pass = 0;
     if (++p.nb < a.nblocks) return;
     p.nb = 0;
@@ -352,7 +395,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
   int to_fetch = count;
   const unsigned char *next_w = nullptr, *next_s = nullptr, *next_z = nullptr;
   auto aim = [&]() {
-    const size_t block = (size_t)s_expert[next.i] * a.nblocks + next.nb;
+    const size_t block = (size_t)s.expert[next.i] * a.nblocks + next.nb;
     next_w = a.weight + (block * a.chunks + next.c) * kTileBytes + lane * 16;
     next_s = a.scales + block * a.G * 64 + g * 8;
     if (ZEROS) next_z = a.zeros + block * a.G * 16 + g * 4;
@@ -377,8 +420,10 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   if (count > 0) aim();
-#pragma unroll
+#pragma unroll 1
   for (int d = 0; d < kDepth; ++d) fetch(d * St::kBytes);
+  w4_join<DT>(a, s, 0);
+  __syncthreads();
 
   float acc[2][4];
   const unsigned char* xp = nullptr;
@@ -386,11 +431,11 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
   int c_first = here.c;      // the warp's first tile of the unit
   auto begin = [&]() {
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[s][i] = 0.0f;
+      for (int i = 0; i < 4; ++i) acc[h][i] = 0.0f;
     // columns behind the unit's last row multiply that row again; their results are dropped
-    const int row = s_lo[here.i] + min(here.pass * 8 + g, s_n[here.i] - 1);
+    const int row = s.lo[here.i] + min(here.pass * 8 + g, s.n[here.i] - 1);
     xp = a.x + ((size_t)row * a.K + here.c * 128 + 8 * j) * 2;
     c_first = here.c;
   };
@@ -399,47 +444,45 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
     if (!Ty::kExact) {
       float probe = 0.0f;  // not finite if any of the sums is not
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) probe = fmaf(0.0f, acc[s][i], probe);
+        for (int i = 0; i < 4; ++i) probe = fmaf(0.0f, acc[h][i], probe);
       if (__any_sync(kFull, probe != 0.0f)) {
-        const size_t block = (size_t)s_expert[here.i] * a.nblocks + here.nb;
-        const int row = s_lo[here.i] + min(here.pass * 8 + g, s_n[here.i] - 1);
+        const size_t block = (size_t)s.expert[here.i] * a.nblocks + here.nb;
+        const int row = s.lo[here.i] + min(here.pass * 8 + g, s.n[here.i] - 1);
         float again[2][4];  // its address leaves the function; acc's must not, or it would not stay in registers
         w4_again<DT, SPAN, ZEROS>(a, block, c_first, here.c, a.x + (size_t)row * a.K * 2, lane, again);
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[s][i] = again[s][i];
+          for (int i = 0; i < 4; ++i) acc[h][i] = again[h][i];
       }
     }
   };
   auto write = [&]() {
-    const int r0 = here.pass * 8, rows = s_n[here.i] - r0, cols = a.N - here.nb * 32 - g;
-    uint16_t* o = reinterpret_cast<uint16_t*>(a.out) + (size_t)(s_lo[here.i] + r0 + 2 * j) * a.N + here.nb * 32 + g;
+    const int r0 = here.pass * 8, rows = s.n[here.i] - r0, cols = a.N - here.nb * 32 - g;
+    uint16_t* o = reinterpret_cast<uint16_t*>(a.out) + (size_t)(s.lo[here.i] + r0 + 2 * j) * a.N + here.nb * 32 + g;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (2 * j + (i & 1) < rows && 16 * s + 8 * (i >> 1) < cols) o[(size_t)(i & 1) * a.N + 16 * s + 8 * (i >> 1)] = Ty::round(acc[s][i]);
+        if (2 * j + (i & 1) < rows && 16 * h + 8 * (i >> 1) < cols) o[(size_t)(i & 1) * a.N + 16 * h + 8 * (i >> 1)] = Ty::round(acc[h][i]);
   };
-  auto leave = [&]() {
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s_sum[warp][(4 * s + i) * 32 + lane] = acc[s][i];
-  };
-
-  if (count > 0) begin();
-  int slot = 0;  // byte offset in the ring
+  int what = 0, slot = 0;  // byte offset in the ring
   for (int t = count; t > 0;) {
+    begin();
     // the rest of this unit, or of the share
-    const int run = min(t, a.chunks - here.c);
-    t -= run;
-    for (const int c_end = here.c + run; here.c < c_end; ++here.c) {
+    const int stretch = min(t, a.chunks - here.c);
+    t -= stretch;
+    uint4 x_next[4];
+    w4_load_x(a, xp, here.c, x_next);
+#pragma unroll 1
+    for (const int c_end = here.c + stretch; here.c < c_end; ++here.c) {
       uint4 x[4], w[4];
-      w4_load_x(a, xp, here.c, x);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[q] = x_next[q];
       xp += 256;
+      if (here.c + 1 < c_end) w4_load_x(a, xp, here.c + 1, x_next);
       asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
       __syncwarp();  // the scales of a tile are copied by all lanes
       const unsigned char* st = ring_p + slot;
@@ -464,42 +507,33 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
           [&](int k, int i) { return Ty::zero_operand((zp[k] >> (4 * i)) & 15u); }, acc);
     }
     finish();
+    const bool ended = here.c == a.chunks;
+    if (began && ended) {
+      write();
+    } else {
+      float* to = s.sum[began ? kW4Warps + warp : warp];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[(2 * j + (i & 1)) * 32 + 16 * h + 8 * (i >> 1) + g] = acc[h][i];
+      what |= began ? kBegins : ended ? kContinues | kEnds : kContinues;
+    }
     if (t > 0) {
-      if (began)
-        write();
-      else
-        leave();
       next_unit(here);
       began = true;
-      begin();
     }
   }
-  // the last unit: finished or not, begun here or not
-  if (count > 0 && !began) leave();
+  if (lane == 0) {
+    s.what[warp] = what;
+    s.place[warp] = here;
+  }
   __syncthreads();
-  if (count > 0 && began) {
-    int64_t end = t_first + count;                          // tiles of the run that are in acc
-    const int64_t unit_end = end + (a.chunks - here.c);
-    for (int w = warp + 1; end < unit_end; ++w) {            // the warps that have the rest of the unit
-      const int64_t w_end = tiles * (w + 1) / kW4Warps;
-      if (w_end > end) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[s][i] = __fadd_rn(acc[s][i], s_sum[w][(4 * s + i) * 32 + lane]);
-        end = w_end;
-      }
-    }
-    write();
-  }
+  w4_join<DT>(a, s, INT_MAX);
 
   // rows of no expert
-  if (first_row > a.rows) first_row = a.rows;
-  if (last_row < first_row) last_row = first_row;
-  const int64_t before = first_row * a.N;
-  const int64_t idle = before + (last_row < a.rows ? (a.rows - last_row) * a.N : 0);
+  const int64_t before = (int64_t)first_row * a.N, idle = before + (a.rows - last_row) * a.N;
   for (int64_t k = (int64_t)blockIdx.x * kW4Threads + tid; k < idle; k += (int64_t)gridDim.x * kW4Threads)
-    reinterpret_cast<uint16_t*>(a.out)[k < before ? k : last_row * a.N + (k - before)] = 0;
+    reinterpret_cast<uint16_t*>(a.out)[k < before ? k : (int64_t)last_row * a.N + (k - before)] = 0;
 }
 
 template <int DT, int SPAN, bool ZEROS>
@@ -531,8 +565,8 @@ extern "C" int moe_rd_expert_matvec_w4(int64_t rows, int32_t N, int32_t K, int32
   if (rows < 0 || rows > (1 << 30) || N < 1 || N > (1 << 24) || K < 32 || K > (1 << 20) || E < 1 || E > kMaxE ||
       group < 32 || group % 32 != 0 || K % group != 0 || (offsets == nullptr && E != 1))
     return MOE_RD_E_SHAPE;
-  // a warp counts its tiles in 32 bits
-  if ((rows / 8 + E) * ((N + 31) / 32) > ((int64_t)1 << 40) / ((K + 127) / 128)) return MOE_RD_E_TOO_LARGE;
+  // tiles are counted in 32 bits
+  if ((rows / 8 + E) * ((N + 31) / 32) > 0x7fffffff / ((K + 127) / 128)) return MOE_RD_E_TOO_LARGE;
   if (rows == 0) return MOE_RD_OK;
   if (x == nullptr || weight == nullptr || scales == nullptr || out == nullptr) return MOE_RD_E_NULL;
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(scales) |
