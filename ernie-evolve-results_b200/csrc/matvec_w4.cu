@@ -28,6 +28,8 @@
 // cut ones (at most its first and its last) in shared memory, where after a barrier they are added in the warps' order.
 #include <limits.h>
 
+#include <atomic>
+
 #include "row_types.cuh"
 
 namespace moe_rd {
@@ -539,9 +541,16 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
 template <int DT, int SPAN, bool ZEROS>
 cudaError_t launch_w4(const W4Args& a, cudaStream_t s) {
   constexpr int smem = kW4Warps * kDepth * W4Stage<SPAN, ZEROS>::kBytes;
-  // per device, and cheap: the attribute is set before every launch, so no state is kept
-  const cudaError_t e = cudaFuncSetAttribute(w4_kernel<DT, SPAN, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> set{0};  // devices whose kernel has its shared memory; setting it twice does no harm
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!((set.load(std::memory_order_relaxed) >> dev) & 1)) {
+    e = cudaFuncSetAttribute(w4_kernel<DT, SPAN, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    set.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
+  }
   return launch_pdl(w4_kernel<DT, SPAN, ZEROS>, dim3((unsigned)device_sms()), dim3(kW4Threads), smem, s, a);
 }
 

@@ -6,6 +6,7 @@ calling into it without a CUDA device, raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 from pathlib import Path
 
 import torch
@@ -176,6 +177,7 @@ def launch_count() -> int:
     return int(lib().moe_rd_launch_count())
 
 
+@functools.lru_cache(maxsize=256)
 def sort_workspace_bytes(T: int, E: int, K: int) -> int:
     n = ctypes.c_size_t(0)
     check(lib().moe_rd_sort_workspace_bytes(T, E, K, ctypes.byref(n)))

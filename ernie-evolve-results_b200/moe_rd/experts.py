@@ -8,7 +8,7 @@ import torch
 
 from . import _cabi
 from ._cabi import ROW_DTYPE
-from .sorting import _aligned, _check_offsets, _ptr, call, check_device, check_out, wants_grad
+from .sorting import _aligned, _check_offsets, _ptr, call, check_device, check_out, spans, wants_grad
 
 
 class W4Weights(NamedTuple):
@@ -94,30 +94,29 @@ def expert_matvec_w4(x: torch.Tensor, weights: W4Weights, offsets: Optional[torc
         raise TypeError("expert_matvec_w4: rows must be bfloat16 or float16")
     if weights.scales.dtype != x.dtype:
         raise TypeError("expert_matvec_w4: rows and scales must have one type")
-    N, K = weights.N, weights.K
-    E, blocks, chunks = weights.packed.shape[:3]
-    G = K // weights.group
+    packed, scales, zeros, N, K, group = weights
+    E, blocks, chunks = packed.shape[:3]
+    G = K // group
     if x.dim() != 2 or x.shape[1] != K:
         raise ValueError(f"expert_matvec_w4: rows must be [R, {K}]")
-    if (weights.packed.shape != (E, -(-N // 32), -(-K // 128), 2048) or weights.packed.dtype != torch.uint8
-            or weights.scales.shape != (E, blocks, G, 8, 4) or not weights.packed.is_contiguous() or not weights.scales.is_contiguous()
-            or (weights.zeros is not None and (weights.zeros.shape != (E, blocks, G, 8, 2) or weights.zeros.dtype != torch.uint8
-                                               or not weights.zeros.is_contiguous()))):
+    if (packed.shape != (E, -(-N // 32), -(-K // 128), 2048) or packed.dtype != torch.uint8 or not packed.is_contiguous()
+            or scales.shape != (E, blocks, G, 8, 4) or not scales.is_contiguous()
+            or (zeros is not None and (zeros.shape != (E, blocks, G, 8, 2) or zeros.dtype != torch.uint8 or not zeros.is_contiguous()))):
         raise ValueError("expert_matvec_w4: weights are not as pack_w4 returns them")
     _check_offsets("expert_matvec_w4", offsets)
     if offsets is None and E != 1:
         raise ValueError("expert_matvec_w4: offsets are needed where there is more than one expert")
     if offsets is not None and offsets.numel() != E + 1:
         raise ValueError(f"expert_matvec_w4: offsets must have {E + 1} elements")
-    if wants_grad(x, weights.scales):
+    if wants_grad(x, scales):
         raise RuntimeError("expert_matvec_w4 is for inference and has no gradient: pass detached rows")
-    dev = check_device("expert_matvec_w4", x, weights.packed, weights.scales, weights.zeros, offsets)
+    dev = check_device("expert_matvec_w4", x, packed, scales, zeros, offsets)
     x2 = _aligned(x)
     R = x.shape[0]
     if out is None:
         out = torch.empty((R, N), dtype=x.dtype, device=dev)
     else:
-        check_out("expert_matvec_w4", out, (R, N), x.dtype, dev, x2)
-    call(dev, _cabi.lib().moe_rd_expert_matvec_w4, R, N, K, E, weights.group, ROW_DTYPE[x.dtype], _ptr(x2), _ptr(weights.packed),
-         _ptr(weights.scales), _ptr(weights.zeros), _ptr(offsets), _ptr(out))
+        check_out("expert_matvec_w4", out, (R, N), x.dtype, dev, spans(x2, packed, scales, zeros, offsets))
+    call(dev, _cabi.lib().moe_rd_expert_matvec_w4, R, N, K, E, group, ROW_DTYPE[x.dtype], _ptr(x2), _ptr(packed), _ptr(scales),
+         _ptr(zeros), _ptr(offsets), _ptr(out))
     return out

@@ -47,29 +47,40 @@ def check_device(name: str, *tensors: Optional[torch.Tensor]) -> torch.device:
 
 def call(dev: torch.device, entry, *args) -> None:
     """Enqueue a C entry point on the current stream of ``dev``."""
-    if dev.index == torch.cuda.current_device():
-        _cabi.check(entry(*args, torch.cuda.current_stream(dev).cuda_stream))
+    index = dev.index
+    if index == torch.cuda.current_device():
+        code = entry(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            _cabi.check(entry(*args, torch.cuda.current_stream(dev).cuda_stream))
+            code = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        _cabi.check(code)
 
 
-def check_out(name: str, out: torch.Tensor, shape, dtype, dev: torch.device, *inputs: Optional[torch.Tensor]) -> torch.Tensor:
-    """``out`` is a buffer the call may write: of this shape and type, contiguous, apart from the inputs."""
-    if out.shape != torch.Size(shape) or out.dtype != dtype or out.device != dev or not out.is_contiguous():
-        raise ValueError(f"{name}: out must be a contiguous {dtype} tensor of shape {tuple(shape)} on {dev}")
-    if out.requires_grad:
-        raise ValueError(f"{name}: out must not require a gradient")
+def spans(*tensors: Optional[torch.Tensor]):
+    """The address ranges of dense tensors."""
+    return [(p, p + t.nbytes) for t in tensors if t is not None and (p := t.data_ptr())]
+
+
+def check_out(name: str, out: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, dev: torch.device, inputs, align: int = 1) -> None:
+    """``out`` is a buffer the call may write: of this shape and type, contiguous, apart from the inputs (``spans``)."""
+    if out.shape != shape or out.dtype != dtype or out.device != dev or not out.is_contiguous() or out.requires_grad:
+        raise ValueError(f"{name}: out must be a contiguous {dtype} tensor of shape {tuple(shape)} on {dev} that needs no gradient")
     lo = out.data_ptr()
-    hi = lo + out.numel() * out.element_size()
-    for t in inputs:
-        if t is not None and lo < hi and t.numel() and t.data_ptr() < hi and lo < t.data_ptr() + t.numel() * t.element_size():
+    if lo % align:
+        raise ValueError(f"{name}: out must be {align}-byte aligned")
+    hi = lo + out.nbytes
+    for begin, end in inputs:
+        if lo < end and begin < hi:
             raise ValueError(f"{name}: out must not share memory with an input")
-    return out
 
 
 def wants_grad(*tensors: Optional[torch.Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _not_while_capturing(name: str, instead: str) -> None:
@@ -109,18 +120,19 @@ def _sort(x, expert_ids, num_experts, capacity, out):
     T, K = expert_ids.shape
     E = num_experts
     dev = x.device
-    x2 = _aligned(x.reshape(T, H))
+    x2 = _aligned(x if x.dim() == 2 else x.reshape(T, H))
     ids = expert_ids.contiguous()
     R = min(T * K, E * capacity) if capacity else T * K
     if out is None:
-        new = lambda *shape, dtype=torch.int32: torch.empty(shape, dtype=dtype, device=dev)  # noqa: E731
-        out = SortedTokens(new(R, H, dtype=x.dtype), new(E + 1), new(T, K), new(R), new(E))
+        offsets, inv, row_token, counts = torch.empty(2 * E + 1 + T * K + R, dtype=torch.int32, device=dev).split((E + 1, T * K, R, E))
+        out = SortedTokens(torch.empty((R, H), dtype=x.dtype, device=dev), offsets, inv.view(T, K), row_token, counts)
     else:
-        check_out("sort_tokens", out.rows, (R, H), x.dtype, dev, x2, ids)
-        for t, shape in ((out.offsets, (E + 1,)), (out.inverse_perm, (T, K)), (out.row_token, (R,)), (out.counts, (E,))):
-            check_out("sort_tokens", t, shape, torch.int32, dev, ids)
-        if out.rows.data_ptr() % 16:
-            raise ValueError("sort_tokens: out.rows must be 16-byte aligned")
+        given = spans(x2, ids)
+        check_out("sort_tokens", out.rows, (R, H), x.dtype, dev, given, 16)
+        check_out("sort_tokens", out.offsets, (E + 1,), torch.int32, dev, given)
+        check_out("sort_tokens", out.inverse_perm, (T, K), torch.int32, dev, given)
+        check_out("sort_tokens", out.row_token, (R,), torch.int32, dev, given)
+        check_out("sort_tokens", out.counts, (E,), torch.int32, dev, given)
     ws_bytes = _cabi.sort_workspace_bytes(T, E, K)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     call(dev, _cabi.lib().moe_rd_sort_tokens, T, H, E, K, ROW_DTYPE[x.dtype], capacity, R, _ptr(x2), _ptr(ids), _ptr(out.rows),
@@ -195,16 +207,14 @@ def _unsort(y, inverse_perm, weights, shared, out):
     H = y.shape[-1]
     T, K = inverse_perm.shape
     dev = y.device
-    y2 = _aligned(y.reshape(-1, H))
+    y2 = _aligned(y if y.dim() == 2 else y.reshape(-1, H))
     inv = inverse_perm.contiguous()
     w = None if weights is None else weights.contiguous()
-    sh = None if shared is None else _aligned(shared.reshape(T, H))
+    sh = None if shared is None else _aligned(shared if shared.dim() == 2 else shared.reshape(T, H))
     if out is None:
         out = torch.empty((T, H), dtype=y.dtype, device=dev)
     else:
-        check_out("unsort_tokens", out, (T, H), y.dtype, dev, y2, inv, w, sh)
-        if out.data_ptr() % 16:
-            raise ValueError("unsort_tokens: out must be 16-byte aligned")
+        check_out("unsort_tokens", out, (T, H), y.dtype, dev, spans(y2, inv, w, sh), 16)
     call(dev, _cabi.lib().moe_rd_unsort_tokens, T, H, K, ROW_DTYPE[y.dtype], _ptr(y2), y2.shape[0], _ptr(inv), _ptr(w),
          _ptr(sh), _ptr(out))
     return out
@@ -271,8 +281,8 @@ def _unsort_backward(grad_out, y, y_shape, inverse_perm, weights, offsets, need_
     for n in y_shape[:-1]:
         R *= n
     dev = grad_out.device
-    g = _aligned(grad_out.reshape(T, H))
-    y2 = _aligned(y.reshape(R, H)) if need_w else None
+    g = _aligned(grad_out if grad_out.dim() == 2 else grad_out.reshape(T, H))
+    y2 = None if not need_w else _aligned(y if y.dim() == 2 else y.reshape(R, H))
     inv = inverse_perm.contiguous()
     w = None if weights is None else weights.contiguous()
     if out is None:
@@ -281,12 +291,11 @@ def _unsort_backward(grad_out, y, y_shape, inverse_perm, weights, offsets, need_
     else:
         if (out.rows is not None) != need_y or (out.weights is not None) != need_w:
             raise ValueError("unsort_tokens_backward: out must hold the gradients that are asked for")
+        given = spans(g, y2, inv, w, offsets)
         if need_y:
-            check_out("unsort_tokens_backward", out.rows, y_shape, g.dtype, dev, g, y2, inv, w)
-            if out.rows.data_ptr() % 16:
-                raise ValueError("unsort_tokens_backward: out.rows must be 16-byte aligned")
+            check_out("unsort_tokens_backward", out.rows, y_shape, g.dtype, dev, given, 16)
         if need_w:
-            check_out("unsort_tokens_backward", out.weights, (T, K), torch.float32, dev, g, y2, inv, w)
+            check_out("unsort_tokens_backward", out.weights, (T, K), torch.float32, dev, given)
     n_rows = None if offsets is None else offsets.data_ptr() + 4 * (offsets.numel() - 1)
     call(dev, _cabi.lib().moe_rd_unsort_tokens_backward, T, H, K, ROW_DTYPE[g.dtype], _ptr(g), _ptr(y2), R, _ptr(inv), _ptr(w),
          n_rows, _ptr(out.rows), _ptr(out.weights))
@@ -376,7 +385,7 @@ def routing_weights(logits: torch.Tensor, expert_ids: torch.Tensor, bias: Option
     if out is None:
         out = torch.empty(expert_ids.shape, dtype=torch.float32, device=dev)
     else:
-        check_out("routing_weights", out, expert_ids.shape, torch.float32, dev, logits, expert_ids, bias)
+        check_out("routing_weights", out, expert_ids.shape, torch.float32, dev, spans(logits, expert_ids, bias))
     _weights_call(_cabi.lib().moe_rd_routing_weights, logits, expert_ids, bias, *config, out)
     return out
 
@@ -396,7 +405,7 @@ def routing_weights_backward(grad_weights: torch.Tensor, logits: torch.Tensor, e
     if out is None:
         out = torch.empty(logits.shape, dtype=torch.float32, device=dev)
     else:
-        check_out("routing_weights_backward", out, logits.shape, torch.float32, dev, logits, expert_ids, bias, grad)
+        check_out("routing_weights_backward", out, logits.shape, torch.float32, dev, spans(logits, expert_ids, bias, grad))
     _weights_call(_cabi.lib().moe_rd_routing_weights_backward, logits, expert_ids, bias, bias_mode, score_fn, renorm, routed_scale,
                   norm_min, grad, out)
     return out
