@@ -7,8 +7,9 @@
 // * batch: sort_count_kernel counts the pairs per (tile of 64 tokens, expert) and per (group of 32 tiles, expert);
 //   positions_kernel and scatter_kernel of the routing pipeline (scatter.cu) derive the places from those counts and
 //   copy the rows, each token row read once and stored K times.
-// * few pairs: one kernel.  Every block works out the places of ALL pairs from the ids in shared memory (the same
-//   stable count) and copies its share of the rows, so a decode step pays one launch and needs no workspace.
+// * up to kOncePairs pairs and kOnceBytes of rows: one kernel.  Every block counts ALL pairs by itself (how many of every expert there are, and
+//   how many before its own tokens), ranks its own pairs and copies their rows: the counting is done hundreds of times
+//   over, but from L2 and by blocks that would otherwise wait, and one launch does the work of three.  No workspace.
 #include "row_types.cuh"
 
 namespace moe_rd {
@@ -59,13 +60,19 @@ sort_count_kernel(const int32_t* __restrict__ ids, int64_t T, int E, int K, int 
   }
 }
 
-constexpr int kFewThreads = 256;
-constexpr int kFewWarps = kFewThreads / 32;
-constexpr int kFewPairs = 1024;
-constexpr int kFewChunks = kFewPairs / 32 / kFewWarps;  // chunks of 32 pairs per warp
-static_assert(kMaxE <= kFewThreads, "one expert per thread");
+constexpr int kOnceThreads = 256;
+constexpr int kOnceWarps = kOnceThreads / 32;
+constexpr int kOncePairs = 16384;
+// Rows beyond this leave L2 while they are written, and the batch form's even spread over the SMs counts for more than
+// its two launches (times on the device, one kernel / batch form; the host needs 10 / 20 us to enqueue them): K = 8, H =
+// 7168 bf16: 16 tokens 3.0 / 8.2 us, 256 tokens 9.0 / 14.6, 512 tokens (59 MB) 12.9 / 22.3, 2048 tokens (235 MB) 56.7 /
+// 51.2; K = 2, H = 4096: 1024 tokens 5.8 / 9.0, 4096 tokens (67 MB) 23.1 / 21.7.
+constexpr int64_t kOnceBytes = 72 << 20;
+constexpr int kOnceBlocksPerSm = 4;
+constexpr int kOwnPairs = 256;  // pairs of a block's tokens
+static_assert(kMaxE <= kOnceThreads && kOwnPairs <= kOnceThreads, "one expert, one pair per thread");
 
-struct FewArgs {
+struct OnceArgs {
   const uint4* x;
   const int32_t* ids;
   uint4* rows;
@@ -75,53 +82,46 @@ struct FewArgs {
   int32_t* counts;
   int64_t capacity, out_rows;
   int T, E, K, nvec;
+  int tokens;  // of a block; blockIdx.x: which tokens, blockIdx.y: which part of their rows
 };
 
-__global__ void __launch_bounds__(kFewThreads) sort_few_kernel(const FewArgs a) {
-  extern __shared__ __align__(16) uint16_t s_cc[];  // [chunks][E] pairs per chunk and expert, then the pairs before it
-  __shared__ int s_off[kMaxE], s_place[kFewPairs], s_w[kFewWarps];
+// A unit of the copy: 32 * UV vectors of a row, UV loads in flight per lane.
+template <int UV>
+__global__ void __launch_bounds__(kOnceThreads, kOnceBlocksPerSm) sort_once_kernel(const OnceArgs a) {
+  __shared__ int s_before[kMaxE], s_after[kMaxE];  // pairs per expert before the block's own, and from them on
+  __shared__ int s_off[kMaxE], s_own[kOwnPairs], s_place[kOwnPairs], s_w[kOnceWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int P = a.T * a.K;
-  const int nch = (P + 31) >> 5;
-  for (int i = tid; i < (nch * a.E + 1) >> 1; i += kFewThreads) reinterpret_cast<uint32_t*>(s_cc)[i] = 0u;
+  s_before[tid] = s_after[tid] = 0;
   __syncthreads();
   pdl_sync();
+  const int t0 = blockIdx.x * a.tokens, ntok = min(a.tokens, a.T - t0);
+  const int P = a.T * a.K, p0 = t0 * a.K, own = ntok * a.K;
   // the first unit of x is on its way while the places are worked out
-  const int upr = (a.nvec + 31) >> 5;  // a unit: 32 vectors of a row
-  const int units = a.T * upr;
-  const int first = blockIdx.x * kFewWarps + warp;
-  const int W = gridDim.x * kFewWarps;
-  uint4 val = make_uint4(0u, 0u, 0u, 0u);
-  if (first < units) {
-    const int t = first / upr, v = (first - t * upr) * 32 + lane;
-    if (v < a.nvec) val = __ldg(a.x + (size_t)t * a.nvec + v);
-  }
-  int e_reg[kFewChunks];
-  unsigned before[kFewChunks];
+  const int upr = (a.nvec + 32 * UV - 1) / (32 * UV);
+  const int units = ntok * upr;
+  const int first = blockIdx.y * kOnceWarps + warp, W = gridDim.y * kOnceWarps;
+  const uint4* x = a.x + (size_t)t0 * a.nvec;
+  uint4 val[UV];
+  auto load = [&](int u) {
+    const int t = u / upr, v = (u - t * upr) * 32 * UV + lane;
 #pragma unroll
-  for (int i = 0; i < kFewChunks; ++i) {
-    const int p = (i * kFewWarps + warp) * 32 + lane;
-    const int e = p < P ? __ldg(a.ids + p) : -1;
-    e_reg[i] = (unsigned)e < (unsigned)a.E ? e : -1;
-  }
+    for (int i = 0; i < UV; ++i)
+      if (v + 32 * i < a.nvec) val[i] = __ldg(x + (size_t)t * a.nvec + v + 32 * i);
+  };
+  if (first < units) load(first);
+  for (int c0 = tid; c0 < P; c0 += 8 * kOnceThreads) {
+    int e[8];
 #pragma unroll
-  for (int i = 0; i < kFewChunks; ++i) {
-    const int c = i * kFewWarps + warp;
-    if (c < nch) {
-      const unsigned m = __match_any_sync(kFull, e_reg[i]);
-      before[i] = __popc(m & ((1u << lane) - 1u));
-      if (e_reg[i] >= 0 && before[i] == 0) s_cc[c * a.E + e_reg[i]] = (uint16_t)__popc(m);
+    for (int i = 0; i < 8; ++i) e[i] = c0 + i * kOnceThreads < P ? __ldg(a.ids + c0 + i * kOnceThreads) : -1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int p = c0 + i * kOnceThreads;
+      if ((unsigned)e[i] < (unsigned)a.E) atomicAdd((p < p0 ? s_before : s_after) + e[i], 1);
+      if ((unsigned)(p - p0) < (unsigned)own) s_own[p - p0] = e[i];
     }
   }
   __syncthreads();
-  int total = 0;
-  if (tid < a.E) {
-    for (int c = 0; c < nch; ++c) {
-      const int v = s_cc[c * a.E + tid];
-      s_cc[c * a.E + tid] = (uint16_t)total;
-      total += v;
-    }
-  }
+  const int total = s_before[tid] + s_after[tid];
   const int kept = a.capacity > 0 && (int64_t)total > a.capacity ? (int)a.capacity : total;
   int incl = kept;
 #pragma unroll
@@ -133,54 +133,53 @@ __global__ void __launch_bounds__(kFewThreads) sort_few_kernel(const FewArgs a) 
   __syncthreads();
   int off = incl - kept, all = 0;
 #pragma unroll
-  for (int w = 0; w < kFewWarps; ++w) {
+  for (int w = 0; w < kOnceWarps; ++w) {
     const int v = s_w[w];
     if (w < warp) off += v;
     all += v;
   }
-  if (tid < a.E) s_off[tid] = off;
-  if (blockIdx.x == 0) {
+  s_off[tid] = off;
+  if (blockIdx.x == 0 && blockIdx.y == 0) {
     if (tid < a.E) {
       a.offsets[tid] = off;
       if (a.counts != nullptr) a.counts[tid] = total;
     }
     if (tid == 0) a.offsets[a.E] = all;
-    for (int64_t r = (int64_t)all + tid; r < a.out_rows; r += kFewThreads) a.row_token[r] = -1;
   }
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kFewChunks; ++i) {
-    const int c = i * kFewWarps + warp, p = c * 32 + lane;
-    if (p < P) {
-      int place = -1;
-      if (e_reg[i] >= 0) {
-        const int rank = s_cc[c * a.E + e_reg[i]] + before[i];
-        if (a.capacity == 0 || rank < a.capacity) place = s_off[e_reg[i]] + rank;
-      }
-      s_place[p] = place;
-      if (blockIdx.x == 0) {
-        a.inverse_perm[p] = place;
-        if (place >= 0) a.row_token[place] = p / a.K;
-      }
+  // a pair's rank among its expert's: those before the block's own, and those before it among these
+  if (tid < own) {
+    const int e = s_own[tid];
+    int place = -1;
+    if ((unsigned)e < (unsigned)a.E) {
+      int rank = s_before[e];
+      for (int q = 0; q < tid; ++q) rank += s_own[q] == e;
+      if (a.capacity == 0 || rank < a.capacity) place = s_off[e] + rank;
+    }
+    s_place[tid] = place;
+    if (blockIdx.y == 0) {
+      a.inverse_perm[p0 + tid] = place;
+      if (place >= 0) a.row_token[place] = t0 + tid / a.K;
     }
   }
   __syncthreads();
   for (int u = first; u < units; u += W) {
-    const int t = u / upr, v = (u - t * upr) * 32 + lane;
-    if (v < a.nvec) {
-      if (u != first) val = __ldg(a.x + (size_t)t * a.nvec + v);
-      for (int k = 0; k < a.K; ++k) {
-        const int place = s_place[t * a.K + k];
-        if (place >= 0) __stcs(a.rows + (size_t)place * a.nvec + v, val);
-      }
+    const int t = u / upr, v = (u - t * upr) * 32 * UV + lane;
+    if (u != first) load(u);
+    for (int k = 0; k < a.K; ++k) {
+      const int place = s_place[t * a.K + k];
+      if (place < 0) continue;
+      uint4* to = a.rows + (size_t)place * a.nvec + v;
+#pragma unroll
+      for (int i = 0; i < UV; ++i)
+        if (v + 32 * i < a.nvec) __stcs(to + 32 * i, val[i]);
     }
   }
-  const int64_t tail = (a.out_rows - all) * upr;
-  for (int64_t u = first; u < tail; u += W) {
-    const int64_t r = u / upr;
-    const int v = (int)(u - r * upr) * 32 + lane;
-    if (v < a.nvec) __stcs(a.rows + (size_t)(all + r) * a.nvec + v, make_uint4(0u, 0u, 0u, 0u));
-  }
+  // rows of nobody
+  const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, blocks = (int64_t)gridDim.x * gridDim.y;
+  for (int64_t r = (int64_t)all + block * kOnceThreads + tid; r < a.out_rows; r += blocks * kOnceThreads) a.row_token[r] = -1;
+  for (int64_t k = ((int64_t)all * a.nvec) + block * kOnceThreads + tid; k < a.out_rows * a.nvec; k += blocks * kOnceThreads)
+    __stcs(a.rows + k, make_uint4(0u, 0u, 0u, 0u));
 }
 
 struct SortWorkspace {
@@ -196,6 +195,8 @@ SortWorkspace carve_sort(int64_t T, int32_t E) {
   return w;
 }
 
+bool in_one_kernel(int64_t T, int32_t H16, int32_t K) { return T * K <= kOncePairs && T * K * H16 * 2 <= kOnceBytes; }
+
 int check_experts(int64_t T, int32_t E) {
   if (E < 1 || E > kMaxE) return MOE_RD_E_SHAPE;
   if ((T + kTile - 1) / kTile * E > 0x7fffffff) return MOE_RD_E_TOO_LARGE;
@@ -207,12 +208,12 @@ int check_experts(int64_t T, int32_t E) {
 
 using namespace moe_rd;
 
-extern "C" int moe_rd_sort_workspace_bytes(int64_t T, int32_t E, int32_t K, size_t* bytes) {
+extern "C" int moe_rd_sort_workspace_bytes(int64_t T, int32_t H, int32_t E, int32_t K, int32_t dtype, size_t* bytes) {
   if (bytes == nullptr) return MOE_RD_E_NULL;
-  int rc = check_rows(T, 8, K, MOE_RD_T_BF16, 0);
+  int rc = check_rows(T, H, K, dtype, 0);
   if (rc == MOE_RD_OK) rc = check_experts(T, E);
   if (rc != MOE_RD_OK) return rc;
-  *bytes = T * K <= kFewPairs ? 0 : carve_sort(T, E).total;
+  *bytes = T == 0 || in_one_kernel(T, dtype == MOE_RD_T_F32 ? 2 * H : H, K) ? 0 : carve_sort(T, E).total;
   return MOE_RD_OK;
 }
 
@@ -236,8 +237,8 @@ extern "C" int moe_rd_sort_tokens(int64_t T, int32_t H, int32_t E, int32_t K, in
     if (e == cudaSuccess && counts != nullptr) e = cudaMemsetAsync(counts, 0, (size_t)E * 4, s);
     if (e == cudaSuccess && out_rows > 0) e = cudaMemsetAsync(row_token, 0xff, (size_t)out_rows * 4, s);
     if (e == cudaSuccess && out_rows > 0) e = cudaMemsetAsync(rows, 0, (size_t)out_rows * H16 * 2, s);
-  } else if (T * K <= kFewPairs) {
-    FewArgs a = {};
+  } else if (in_one_kernel(T, H16, K)) {
+    OnceArgs a = {};
     a.x = static_cast<const uint4*>(x);
     a.ids = expert_ids;
     a.rows = static_cast<uint4*>(rows);
@@ -251,10 +252,19 @@ extern "C" int moe_rd_sort_tokens(int64_t T, int32_t H, int32_t E, int32_t K, in
     a.E = E;
     a.K = K;
     a.nvec = H16 / 8;
-    const int64_t want = (T * ((a.nvec + 31) / 32) + kFewWarps - 1) / kFewWarps;
-    const int64_t cap = (int64_t)device_sms() * 2;
-    const size_t smem = (size_t)((T * K + 31) / 32) * E * 2 + 16;
-    e = launch_pdl(sort_few_kernel, dim3((unsigned)(want < cap ? want : cap)), dim3(kFewThreads), smem, s, a);
+    // as many blocks as are resident at once, each with the same number of tokens (at most kOwnPairs pairs: there are
+    // kOncePairs at most); few tokens share their rows' columns out among blocks
+    const int most = device_sms() * kOnceBlocksPerSm;
+    a.tokens = (int)((T + most - 1) / most);
+    while (a.tokens > 1 && a.tokens * K > kOwnPairs) --a.tokens;
+    const int bx = (int)((T + a.tokens - 1) / a.tokens);
+    const int units = (a.nvec + 31) / 32;
+    int by = (a.tokens * units + kOnceWarps - 1) / kOnceWarps;
+    if (by > most / bx) by = most / bx > 1 ? most / bx : 1;
+    // more units than resident warps: fewer and larger ones
+    const dim3 grid((unsigned)bx, (unsigned)by);
+    e = T * units > (int64_t)most * kOnceWarps * 2 ? launch_pdl(sort_once_kernel<4>, grid, dim3(kOnceThreads), 0, s, a)
+                                               : launch_pdl(sort_once_kernel<1>, grid, dim3(kOnceThreads), 0, s, a);
     count_launch();
   } else {
     const SortWorkspace w = carve_sort(T, E);

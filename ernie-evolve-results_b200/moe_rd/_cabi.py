@@ -135,7 +135,7 @@ def lib() -> ctypes.CDLL:
         L.moe_rd_expert_stats.restype = ctypes.c_int
         ptr, i32, i64, f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
         for name, argtypes in (
-                ("moe_rd_sort_workspace_bytes", [i64, i32, i32, ctypes.POINTER(ctypes.c_size_t)]),
+                ("moe_rd_sort_workspace_bytes", [i64, i32, i32, i32, i32, ctypes.POINTER(ctypes.c_size_t)]),
                 ("moe_rd_sort_tokens", [i64, i32, i32, i32, i32, i64, i64] + [ptr] * 8 + [ctypes.c_size_t, ptr]),
                 ("moe_rd_unsort_tokens", [i64, i32, i32, i32, ptr, i64] + [ptr] * 5),
                 ("moe_rd_unsort_tokens_backward", [i64, i32, i32, i32, ptr, ptr, i64] + [ptr] * 6),
@@ -178,7 +178,7 @@ def launch_count() -> int:
 
 
 @functools.lru_cache(maxsize=256)
-def sort_workspace_bytes(T: int, E: int, K: int) -> int:
+def sort_workspace_bytes(T: int, H: int, E: int, K: int, dtype: int) -> int:
     n = ctypes.c_size_t(0)
-    check(lib().moe_rd_sort_workspace_bytes(T, E, K, ctypes.byref(n)))
+    check(lib().moe_rd_sort_workspace_bytes(T, H, E, K, dtype, ctypes.byref(n)))
     return int(n.value)

@@ -133,7 +133,7 @@ def _sort(x, expert_ids, num_experts, capacity, out):
         check_out("sort_tokens", out.inverse_perm, (T, K), torch.int32, dev, given)
         check_out("sort_tokens", out.row_token, (R,), torch.int32, dev, given)
         check_out("sort_tokens", out.counts, (E,), torch.int32, dev, given)
-    ws_bytes = _cabi.sort_workspace_bytes(T, E, K)
+    ws_bytes = _cabi.sort_workspace_bytes(T, H, E, K, ROW_DTYPE[x.dtype])
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     call(dev, _cabi.lib().moe_rd_sort_tokens, T, H, E, K, ROW_DTYPE[x.dtype], capacity, R, _ptr(x2), _ptr(ids), _ptr(out.rows),
          _ptr(out.offsets), _ptr(out.inverse_perm), _ptr(out.row_token), _ptr(out.counts), _ptr(ws), ws_bytes)

@@ -407,10 +407,11 @@ enum { MOE_RD_T_BF16 = 0, MOE_RD_T_FP16 = 1, MOE_RD_T_F32 = 2 };
  * out_rows: at least T*K, or E*capacity where that is less.  Every output is
  * written whole: rows behind offsets[E] become zero, with row_token -1.
  * E <= 256, K <= 32 (K may exceed E).  Workspace: moe_rd_sort_workspace_bytes
- * bytes, 256-byte aligned; nothing in it has to be initialised.  May be recorded
- * into a CUDA graph.
+ * bytes, 256-byte aligned; nothing in it has to be initialised (a small
+ * sort needs none: 0 bytes, and the pointer may be NULL).  May be recorded into a
+ * CUDA graph.
  */
-int moe_rd_sort_workspace_bytes(int64_t T, int32_t E, int32_t K, size_t* bytes);
+int moe_rd_sort_workspace_bytes(int64_t T, int32_t H, int32_t E, int32_t K, int32_t dtype, size_t* bytes);
 int moe_rd_sort_tokens(int64_t T, int32_t H, int32_t E, int32_t K, int32_t dtype, int64_t capacity,
                        int64_t out_rows, const void* x, const int32_t* expert_ids, void* rows,
                        int32_t* offsets, int32_t* inverse_perm, int32_t* row_token, int32_t* counts,

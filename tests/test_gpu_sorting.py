@@ -57,13 +57,18 @@ SORT_CASES = [
     (1, 1, 1, 8, "bf16", 0, "random"),
     (3, 2, 5, 4, "fp32", 0, "padded"),
     (7, 3, 60, 264, "fp16", 1, "random"),
-    (128, 8, 256, 1024, "bf16", 0, "random"),     # 1024 pairs: the last size of the one-kernel form
-    (129, 8, 256, 1024, "bf16", 0, "random"),     # the first of the batch form
+    (2048, 8, 256, 1024, "bf16", 0, "random"),    # 16384 pairs: the last size of the one-kernel form
+    (2049, 8, 256, 1024, "bf16", 0, "random"),    # the first of the batch form
+    (16384, 1, 3, 8, "bf16", 0, "padded"),        # many tokens a block
     (1025, 1, 7, 20, "fp32", 100, "padded"),
     (33, 32, 4, 72, "fp16", 0, "random"),         # more ids than experts: the same expert several times per token
     (64, 32, 256, 40, "bf16", 3, "stray"),
     (2047, 2, 8, 136, "bf16", 300, "one expert"),
-    (2049, 2, 8, 516, "fp32", 0, "stray"),        # one token into a second group of counting tiles
+    (2049, 2, 8, 516, "fp32", 0, "stray"),
+    (2049, 9, 8, 132, "fp32", 0, "stray"),        # one token into a second group of counting tiles
+    (4100, 5, 16, 264, "fp16", 900, "one expert"),
+    (700, 32, 33, 72, "bf16", 0, "padded"),
+    (8200, 2, 16, 64, "bf16", 0, "none"),
     (40, 4, 16, 64, "bf16", 0, "none"),
     (600, 4, 16, 64, "fp16", 2, "none"),
     (5000, 6, 160, 520, "fp16", 200, "padded"),

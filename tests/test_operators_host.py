@@ -110,12 +110,14 @@ def test_c_entries_validate_before_any_cuda_call():
     buf = (ctypes.c_char * 4096)()
     p = (ctypes.addressof(buf) + 255) & ~255
     n = ctypes.c_size_t(7)
-    assert L.moe_rd_sort_workspace_bytes(1, 256, 8, ctypes.byref(n)) == 0 and n.value == 0
-    assert L.moe_rd_sort_workspace_bytes(129, 256, 8, ctypes.byref(n)) == 0 and n.value == 256 * 4 * 3 + 1024
-    assert L.moe_rd_sort_workspace_bytes(1, 257, 8, ctypes.byref(n)) == -2
-    assert L.moe_rd_sort_workspace_bytes(1, 8, 33, ctypes.byref(n)) == -2
-    assert L.moe_rd_sort_workspace_bytes(2 ** 31, 8, 1, ctypes.byref(n)) == -2
-    assert L.moe_rd_sort_workspace_bytes(1, 8, 1, None) == -1
+
+    def ws(T, H=64, E=256, K=8, dtype=0, to=ctypes.byref(n)):
+        return L.moe_rd_sort_workspace_bytes(T, H, E, K, dtype, to)
+    assert ws(1) == 0 and n.value == 0 and ws(2048) == 0 and n.value == 0
+    assert ws(2049) == 0 and n.value == 256 * 4 * 33 + 256 * 4 * 2
+    assert ws(2048, H=7168) == 0 and n.value == 256 * 4 * 32 + 256 * 4 and ws(2 ** 31 - 1, K=1, E=1) == 0
+    assert ws(1, E=257) == ws(1, K=33) == ws(2 ** 31, K=1) == ws(1, H=12) == -2 and ws(1, dtype=3) == -6 and ws(1, to=None) == -1
+    assert ws(2 ** 30, K=1) == -10      # 2^24 tiles x 256 experts are not counted in 32 bits
 
     def sort(T=4, H=64, E=8, K=2, dtype=0, cap=0, R=8, ptrs=(p,) * 7, ws=0, bytes_=0):
         return L.moe_rd_sort_tokens(T, H, E, K, dtype, cap, R, *ptrs, ws, bytes_, None)
@@ -125,7 +127,7 @@ def test_c_entries_validate_before_any_cuda_call():
     for i in (0, 1, 2, 3, 4, 5):
         assert sort(ptrs=tuple(0 if j == i else p for j in range(7))) == -1
     assert sort(ptrs=(p + 8,) + (p,) * 6) == -4
-    assert sort(T=600, R=1200) == sort(T=600, R=1200, ws=p, bytes_=16) == sort(T=600, R=1200, ws=p + 16, bytes_=4000) == -5
+    assert sort(T=9000, R=18000) == sort(T=9000, R=18000, ws=p, bytes_=16) == sort(T=9000, R=18000, ws=p + 16, bytes_=1 << 20) == -5
 
     def unsort(T=4, H=64, K=2, dtype=0, R=8, ptrs=(p, p, p, p, p)):
         return L.moe_rd_unsort_tokens(T, H, K, dtype, ptrs[0], R, *ptrs[1:], None)
