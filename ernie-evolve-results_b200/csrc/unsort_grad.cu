@@ -31,9 +31,11 @@ struct UnsortGradArgs {
   int warps_per_token;    // 1, 2, 4 or 8
 };
 
-// KT slots at a time; NEED_W: grad_weights is wanted (and y is read).
+// KT slots at a time; NEED_W: grad_weights is wanted (and y is read).  The compiler left alone takes 128 registers for
+// KT = 8, two blocks per SM; with 80 and three blocks 32768 tokens x 2048, K = 8 take 364 us instead of 401, and with four
+// warps a token instead of eight 346 us (6.2 TB/s).  KT = 2 is fastest left alone (108 us against 123 for 16384 x 4096).
 template <int DT, int KT, bool NEED_W>
-__global__ void __launch_bounds__(kGradThreads) unsort_grad_kernel(const UnsortGradArgs a) {
+__global__ void __launch_bounds__(kGradThreads, KT == 8 ? 3 : KT == 4 ? 4 : 0) unsort_grad_kernel(const UnsortGradArgs a) {
   constexpr int NE = RowVec<DT>::N;
   __shared__ float s_part[kGradWarps][KT];
   pdl_sync();
@@ -163,7 +165,8 @@ extern "C" int moe_rd_unsort_tokens_backward(int64_t T, int32_t H, int32_t K, in
     a.y_rows = y_rows;
     a.nvec = dtype == MOE_RD_T_F32 ? H / 4 : H / 8;
     a.K = K;
-    a.warps_per_token = a.nvec > 128 ? 8 : a.nvec > 64 ? 4 : a.nvec > 32 ? 2 : 1;
+    // four warps a token at most, eight where there are too few tokens to fill the SMs
+    a.warps_per_token = a.nvec > 128 && T <= 4 * device_sms() ? 8 : a.nvec > 64 ? 4 : a.nvec > 32 ? 2 : 1;
     const int tokens = kGradWarps / a.warps_per_token;
     const int64_t want = (T + tokens - 1) / tokens;
     const int64_t cap = (int64_t)device_sms() * kGradBlocksPerSm;
