@@ -8,17 +8,15 @@
 // integers into its operands:
 //
 // * A tile of 32 outputs x 128 inputs is 2 KB, stored so that a lane's 16-byte loads are its operand fragments: word i
-//   holds the eight inputs 32i + 8j.. of one output, the pair (2p, 2p+1) in its two halves.
-// * bf16: the four bits of pair p are the topmost mantissa bits of each half once the word is rotated by 4p; with the
-//   exponent of 16 that is the pair of numbers 16 + q, one rotation and one LOP3 for two weights.  The matrix
-//   instruction multiplies those, and (16 + zero) * sum of x over the group is subtracted from the group's fp32 sum; the
-//   sums of x come from one more matrix instruction with ones, shared by the tile's 32 outputs.  16 is as small as the
-//   weights themselves, so the subtraction costs a few units of 2^-24 of the sum of the magnitudes.
+//   holds the eight inputs 32i + 8j.. of one output, the pair (2p, 2p+1) in nibble p of its two halves.
+// * bf16: (w >> 4p) & 0x000f000f with the exponent of 128 or'ed in (one LOP3) is the pair 128 + q, from which 128 + zero is
+//   subtracted exactly: q - zero is an integer in -15..15.
 // * fp16: there is room for two nibbles below the exponent, 1024 + q and 1024 + 16 q, from which a subtraction or a fused
-//   multiply-add makes q - zero exactly: half as many shifts.
+//   multiply-add makes q - zero exactly: a third of the shifts.
 // * The scale of a group multiplies its fp32 sum; nothing is rounded below 32 bits before the result is.
-// Infinities: (16 + q) * inf - (16 + zero) * inf is no number where (q - zero) * inf is one.  A warp whose sums are not
-// finite computes its stretch again with q - zero as the operand.
+// Leaving the subtraction to the sums (operands 128 + q or 16 + q, and (16 + zero) * sum of x taken off afterwards) saves a
+// quarter of the instructions and was slower: the sums of x cost matrix instructions, and it is their chains that a warp
+// waits for (8 experts x 8192 outputs x 7168 inputs 51.3 against 50.3 us; groups of 32 64.5 against 54.4 us).
 //
 // A unit of work is 32 outputs of one expert for up to eight of its rows; its tiles lie one behind the other in memory,
 // and so do the units of an expert.  Only experts that have rows get units: every block lists them from the offsets.  A
@@ -40,7 +38,9 @@ namespace {
 
 constexpr int kW4Threads = 512;
 constexpr int kW4Warps = kW4Threads / 32;
-constexpr int kDepth = 4;  // tiles in flight per warp
+// Tiles in flight per warp: 2 KB x 16 warps x 2 is 64 KB an SM, more than a microsecond of its share of the HBM rate.
+// Deeper rings only put off the products: 8 experts x 2048 outputs x 7168 inputs 18.0 us with 2, 19.1 with 3, 19.8 with 4.
+constexpr int kDepth = 2;
 constexpr int kTileBytes = 2048;
 
 struct W4Args {
@@ -85,20 +85,16 @@ struct W4Type;
 
 template <>
 struct W4Type<MOE_RD_T_BF16> {
-  static constexpr bool kExact = false;  // operands are 16 + q
-  uint32_t mask = in_register<0x00780078u>(), base = in_register<0x41804180u>();
+  uint32_t mask = in_register<0x000f000fu>(), base = in_register<0x43004300u>();
   static __device__ __forceinline__ float first(uint32_t v) { return bf16_lo(v); }
   static __device__ __forceinline__ float second(uint32_t v) { return bf16_hi(v); }
-  static __device__ __forceinline__ uint32_t zero_operand(uint32_t zero) { return 0x41804180u | (zero * 0x00080008u); }
-  __device__ __forceinline__ void unpack(uint32_t w, uint32_t, uint32_t (&o)[4]) const {
-#pragma unroll
-    for (int p = 0; p < 4; ++p) o[p] = and_or(p ? __funnelshift_r(w, w, 4 * p) : w, mask, base);
-  }
-  __device__ __forceinline__ void unpack_exact(uint32_t w, uint32_t zero, uint32_t (&o)[4]) const {
-    unpack(w, zero, o);
+  static __device__ __forceinline__ uint32_t zero_operand(uint32_t zero) { return 0x43004300u | (zero * 0x00010001u); }
+  // the four operands q - zero of a word
+  __device__ __forceinline__ void unpack(uint32_t w, uint32_t zero, uint32_t (&o)[4]) const {
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-      const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&o[p]), *reinterpret_cast<const __nv_bfloat162*>(&zero));
+      const uint32_t v = and_or(w >> (4 * p), mask, base);
+      const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&zero));
       o[p] = *reinterpret_cast<const uint32_t*>(&d);
     }
   }
@@ -112,12 +108,10 @@ struct W4Type<MOE_RD_T_BF16> {
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
   }
-  static constexpr uint32_t kOnes = 0x3f803f80u;
 };
 
 template <>
 struct W4Type<MOE_RD_T_FP16> {
-  static constexpr bool kExact = true;  // operands are q - zero
   uint32_t low = in_register<0x000f000fu>(), high = in_register<0x00f000f0u>(), base = in_register<0x64006400u>();
   static __device__ __forceinline__ float first(uint32_t v) { return __low2float(*reinterpret_cast<const __half2*>(&v)); }
   static __device__ __forceinline__ float second(uint32_t v) { return __high2float(*reinterpret_cast<const __half2*>(&v)); }
@@ -135,7 +129,6 @@ struct W4Type<MOE_RD_T_FP16> {
       o[p] = *reinterpret_cast<const uint32_t*>(&d);
     }
   }
-  __device__ __forceinline__ void unpack_exact(uint32_t w, uint32_t zero, uint32_t (&o)[4]) const { unpack(w, zero, o); }
   static __device__ __forceinline__ uint16_t round(float v) { return __half_as_ushort(__float2half_rn(v)); }
   static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                              uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
@@ -143,12 +136,11 @@ struct W4Type<MOE_RD_T_FP16> {
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
   }
-  static constexpr uint32_t kOnes = 0x3c003c00u;
 };
 
-// acc (+)= the product of one tile: w[2s + h] are the words of outputs 16s + 8h + g, x[q] the lane's inputs of block q,
+// acc += the product of one tile: w[2s + h] are the words of outputs 16s + 8h + g, x[q] the lane's inputs of block q,
 // scale(k, i) and zero(k, i) those of group k of the tile and output 8i + g.
-template <int DT, int SPAN, bool EXACT, typename Scale, typename Zero>
+template <int DT, int SPAN, typename Scale, typename Zero>
 __device__ __forceinline__ void w4_tile(const W4Type<DT>& ty, const uint4 (&w)[4], const uint4 (&x)[4], Scale scale, Zero zero,
                                         float (&acc)[2][4]) {
   using Ty = W4Type<DT>;
@@ -156,29 +148,15 @@ __device__ __forceinline__ void w4_tile(const W4Type<DT>& ty, const uint4 (&w)[4
                                {w[2].x, w[2].y, w[2].z, w[2].w}, {w[3].x, w[3].y, w[3].z, w[3].w}};
 #pragma unroll
   for (int k = 0; k < 4 / SPAN; ++k) {
-    float part[2][4], ones[4];
+    float part[2][4];
 #pragma unroll
     for (int q = k * SPAN; q < (k + 1) * SPAN; ++q) {
-      const bool fresh = q == k * SPAN;
-      if (!EXACT) {
-        constexpr uint32_t one = Ty::kOnes;
-        if (fresh)
-          Ty::mma(ones, one, one, one, one, x[q].x, x[q].y, 0.0f, 0.0f, 0.0f, 0.0f);
-        else
-          Ty::mma(ones, one, one, one, one, x[q].x, x[q].y, ones[0], ones[1], ones[2], ones[3]);
-        Ty::mma(ones, one, one, one, one, x[q].z, x[q].w, ones[0], ones[1], ones[2], ones[3]);
-      }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         uint32_t a[4], b[4];
-        if (EXACT) {
-          ty.unpack_exact(word[2 * s][q], zero(k, 2 * s), a);
-          ty.unpack_exact(word[2 * s + 1][q], zero(k, 2 * s + 1), b);
-        } else {
-          ty.unpack(word[2 * s][q], 0u, a);
-          ty.unpack(word[2 * s + 1][q], 0u, b);
-        }
-        if (fresh)
+        ty.unpack(word[2 * s][q], zero(k, 2 * s), a);
+        ty.unpack(word[2 * s + 1][q], zero(k, 2 * s + 1), b);
+        if (q == k * SPAN)
           Ty::mma(part[s], a[0], b[0], a[1], b[1], x[q].x, x[q].y, 0.0f, 0.0f, 0.0f, 0.0f);
         else
           Ty::mma(part[s], a[0], b[0], a[1], b[1], x[q].x, x[q].y, part[s][0], part[s][1], part[s][2], part[s][3]);
@@ -186,14 +164,9 @@ __device__ __forceinline__ void w4_tile(const W4Type<DT>& ty, const uint4 (&w)[4
       }
     }
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float p = part[s][i];
-        if (!EXACT) p = fmaf(-Ty::first(zero(k, 2 * s + (i >> 1))), ones[i & 1], p);
-        acc[s][i] = fmaf(scale(k, 2 * s + (i >> 1)), p, acc[s][i]);
-      }
-    }
+      for (int i = 0; i < 4; ++i) acc[s][i] = fmaf(scale(k, 2 * s + (i >> 1)), part[s][i], acc[s][i]);
   }
 }
 
@@ -219,39 +192,6 @@ __device__ __forceinline__ void w4_load_x(const W4Args& a, const unsigned char* 
 #pragma unroll
     for (int q = 0; q < 4; ++q)
       x[q] = 128 * c + 32 * q < a.K ? __ldg(reinterpret_cast<const uint4*>(xp + 64 * q)) : make_uint4(0u, 0u, 0u, 0u);
-  }
-}
-
-// Tiles [c0, c1) of a unit once more, with q - zero as the operand, straight from global memory.
-template <int DT, int SPAN, bool ZEROS>
-__device__ __noinline__ void w4_again(const W4Args& a, size_t block, int c0, int c1, const unsigned char* x_row, int lane,
-                                      float (&acc)[2][4]) {
-  const W4Type<DT> ty;
-  const int g = lane >> 2, j = lane & 3;
-#pragma unroll
-  for (int s = 0; s < 2; ++s)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[s][i] = 0.0f;
-  for (int c = c0; c < c1; ++c) {
-    uint4 w[4], x[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w[i] = __ldg(reinterpret_cast<const uint4*>(a.weight + (block * a.chunks + c) * kTileBytes + i * 512 + lane * 16));
-    w4_load_x(a, x_row + (size_t)c * 256 + 16 * j, c, x);
-    w4_tile<DT, SPAN, true>(
-        ty, w, x,
-        [&](int k, int i) {
-          const size_t at = block * a.G + w4_group(a, 4 * c + SPAN * k);
-          const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(a.scales + at * 64 + g * 8) + (i >> 1));
-          return i & 1 ? W4Type<DT>::second(v) : W4Type<DT>::first(v);
-        },
-        [&](int k, int i) {
-          if (!ZEROS) return W4Type<DT>::zero_operand(8u);
-          const size_t at = block * a.G + w4_group(a, 4 * c + SPAN * k);
-          const uint32_t v = __ldg(reinterpret_cast<const uint16_t*>(a.zeros + at * 16) + g);
-          return W4Type<DT>::zero_operand((v >> (4 * i)) & 15u);
-        },
-        acc);
   }
 }
 
@@ -430,7 +370,6 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
   float acc[2][4];
   const unsigned char* xp = nullptr;
   bool began = here.c == 0;  // this warp has the unit from its first tile on
-  int c_first = here.c;      // the warp's first tile of the unit
   auto begin = [&]() {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -439,27 +378,6 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
     // columns behind the unit's last row multiply that row again; their results are dropped
     const int row = s.lo[here.i] + min(here.pass * 8 + g, s.n[here.i] - 1);
     xp = a.x + ((size_t)row * a.K + here.c * 128 + 8 * j) * 2;
-    c_first = here.c;
-  };
-  // the sums of tiles [c_first, here.c) of the unit are complete
-  auto finish = [&]() {
-    if (!Ty::kExact) {
-      float probe = 0.0f;  // not finite if any of the sums is not
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) probe = fmaf(0.0f, acc[h][i], probe);
-      if (__any_sync(kFull, probe != 0.0f)) {
-        const size_t block = (size_t)s.expert[here.i] * a.nblocks + here.nb;
-        const int row = s.lo[here.i] + min(here.pass * 8 + g, s.n[here.i] - 1);
-        float again[2][4];  // its address leaves the function; acc's must not, or it would not stay in registers
-        w4_again<DT, SPAN, ZEROS>(a, block, c_first, here.c, a.x + (size_t)row * a.K * 2, lane, again);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[h][i] = again[h][i];
-      }
-    }
   };
   auto write = [&]() {
     const int r0 = here.pass * 8, rows = s.n[here.i] - r0, cols = a.N - here.nb * 32 - g;
@@ -476,18 +394,15 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
     // the rest of this unit, or of the share
     const int stretch = min(t, a.chunks - here.c);
     t -= stretch;
-    uint4 x_next[4];
-    w4_load_x(a, xp, here.c, x_next);
-#pragma unroll 1
-    for (const int c_end = here.c + stretch; here.c < c_end; ++here.c) {
-      uint4 x[4], w[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) x[q] = x_next[q];
+    // one tile with x in `x`, while the x of the next is fetched into `x_next`
+    const int c_end = here.c + stretch;
+    auto tile = [&](const uint4 (&x)[4], uint4 (&x_next)[4]) {
       xp += 256;
       if (here.c + 1 < c_end) w4_load_x(a, xp, here.c + 1, x_next);
       asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
       __syncwarp();  // the scales of a tile are copied by all lanes
       const unsigned char* st = ring_p + slot;
+      uint4 w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4*>(st + i * 512 + lane * 16);
       uint2 sc[St::kParts];
@@ -500,15 +415,24 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
       __syncwarp();
       fetch(slot);
       slot = slot + St::kBytes == kDepth * St::kBytes ? 0 : slot + St::kBytes;
-      w4_tile<DT, SPAN, Ty::kExact>(
+      w4_tile<DT, SPAN>(
           ty, w, x,
           [&](int k, int i) {
             const uint32_t v = i < 2 ? sc[k].x : sc[k].y;
             return i & 1 ? Ty::second(v) : Ty::first(v);
           },
           [&](int k, int i) { return Ty::zero_operand((zp[k] >> (4 * i)) & 15u); }, acc);
+      ++here.c;
+    };
+    uint4 x0[4], x1[4];
+    w4_load_x(a, xp, here.c, x0);
+#pragma unroll 1
+    while (true) {
+      tile(x0, x1);
+      if (here.c == c_end) break;
+      tile(x1, x0);
+      if (here.c == c_end) break;
     }
-    finish();
     const bool ended = here.c == a.chunks;
     if (began && ended) {
       write();

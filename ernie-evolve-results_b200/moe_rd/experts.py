@@ -69,8 +69,6 @@ def pack_w4(q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor]
     packed[..., 1] = (r[..., 2] & 15) | ((r[..., 3] & 15) << 4)
     packed[..., 2] = (r[..., 0] >> 4) | (r[..., 1] & 0xF0)
     packed[..., 3] = (r[..., 2] >> 4) | (r[..., 3] & 0xF0)
-    if scales.dtype == torch.bfloat16:  # rotate every word left by three bits
-        packed = (packed << 3) | (packed.roll(1, -1) >> 5)
     if zeros is not None:
         z = _blocked(zeros)
         zeros = z[..., 0::2] | (z[..., 1::2] << 4)

@@ -487,8 +487,7 @@ int moe_rd_routing_weights_backward(int64_t T, int32_t E, int32_t K, int32_t sco
  * ceil(N/32), G = K/group):
  *   weight [E][B][C][4][32][4] 32-bit words: part i (outputs 32b + 8i + 0..7), lane
  *     4*r + j (output r of the part), word m: the eight inputs 128c + 32m + 8j +
- *     0..7 of that output, input 2p in bits 4p.. and input 2p+1 in bits 16+4p..;
- *     for bf16 the whole word rotated left by three bits
+ *     0..7 of that output, input 2p in bits 4p.. and input 2p+1 in bits 16+4p..
  *   scales [E][B][G][8][4] (outputs r, r + 8, r + 16, r + 24 of the block)
  *   zeros  [E][B][G][8]    16 bits: four bits for each of the same outputs, lowest first
  */

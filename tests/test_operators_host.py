@@ -80,8 +80,6 @@ def test_pack_w4_layout_and_refusals(dtype):
         m, j, kk = (k % 128) // 32, (k % 32) // 8, k % 8
         at = part * 512 + (4 * r + j) * 16 + 4 * m
         word = int.from_bytes(bytes(p.packed[e, b, c, at:at + 4].tolist()), "little")
-        if dtype == torch.bfloat16:
-            word = (word >> 3) | ((word & 7) << 29)
         assert (word >> (4 * (kk // 2) + 16 * (kk % 2))) & 15 == int(value[e, n, k])
         assert p.scales[e, b, k // group, r, part] == s[e, n, k // group]
         word = int.from_bytes(bytes(p.zeros[e, b, k // group, r].tolist()), "little")
