@@ -462,6 +462,28 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
     reinterpret_cast<uint16_t*>(a.out)[k < before ? k : (int64_t)last_row * a.N + (k - before)] = 0;
 }
 
+// The layout of the weights, once when a program loads them: a thread makes one 16-byte vector (four words) of a tile.
+__global__ void __launch_bounds__(256) pack_w4_kernel(const unsigned char* __restrict__ q, uint4* __restrict__ out, int64_t vectors, int N,
+                                                      int half, int blocks, int chunks) {
+  pdl_sync();
+  for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < vectors; v += (int64_t)gridDim.x * 256) {
+    const int lane = (int)(v & 31), part = (int)(v >> 5) & 3;
+    const int64_t tile = v >> 7, eb = tile / chunks, e = eb / blocks;
+    const int c = (int)(tile - eb * chunks), n = (int)(eb - e * blocks) * 32 + part * 8 + (lane >> 2);
+    const unsigned char* row = q + ((size_t)e * N + n) * half;
+    uint32_t o[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const int at = 64 * c + 16 * m + 4 * (lane & 3);
+      const uint32_t w = n < N && at < half ? __ldg(reinterpret_cast<const uint32_t*>(row + at)) : 0u;
+      o[m] = 0u;
+#pragma unroll
+      for (int p = 0; p < 4; ++p) o[m] |= ((w >> (8 * p)) & 15u) << (4 * p) | ((w >> (8 * p + 4)) & 15u) << (16 + 4 * p);
+    }
+    out[v] = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
 template <int DT, int SPAN, bool ZEROS>
 cudaError_t launch_w4(const W4Args& a, cudaStream_t s) {
   constexpr int smem = kW4Warps * kDepth * W4Stage<SPAN, ZEROS>::kBytes;
@@ -489,6 +511,20 @@ cudaError_t launch_w4_span(const W4Args& a, int group, cudaStream_t s) {
 }  // namespace moe_rd
 
 using namespace moe_rd;
+
+extern "C" int moe_rd_pack_w4(int32_t E, int32_t N, int32_t K, const uint8_t* q, void* weight, void* stream) {
+  if (E < 1 || E > kMaxE || N < 1 || N > (1 << 24) || K < 32 || K > (1 << 20) || K % 32 != 0) return MOE_RD_E_SHAPE;
+  if (q == nullptr || weight == nullptr) return MOE_RD_E_NULL;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(weight)) & 15) return MOE_RD_E_ALIGN;
+  const int blocks = (N + 31) / 32, chunks = (K + 127) / 128;
+  const int64_t vectors = (int64_t)E * blocks * chunks * (kTileBytes / 16);
+  const int64_t want = (vectors + 255) / 256, cap = (int64_t)device_sms() * 64;
+  const cudaError_t e = launch_pdl(pack_w4_kernel, dim3((unsigned)(want < cap ? want : cap)), dim3(256), 0, static_cast<cudaStream_t>(stream),
+                                   static_cast<const unsigned char*>(q), static_cast<uint4*>(weight), vectors, (int)N, K / 2, blocks, chunks);
+  count_launch();
+  if (e != cudaSuccess) set_last_cuda_error(e);
+  return e == cudaSuccess ? MOE_RD_OK : MOE_RD_E_CUDA;
+}
 
 extern "C" int moe_rd_expert_matvec_w4(int64_t rows, int32_t N, int32_t K, int32_t E, int32_t group, int32_t dtype,
                                        const void* x, const void* weight, const void* scales, const uint16_t* zeros,

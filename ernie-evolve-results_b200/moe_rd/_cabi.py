@@ -28,7 +28,7 @@ EXPORTS = (
     "moe_rd_combine_add_rows",
     "moe_rd_ep_scatter", "moe_rd_ep_scatter_once", "moe_rd_ep_replicate", "moe_rd_ep_combine", "moe_rd_read_status_noalloc", "moe_rd_gemm_plan", "moe_rd_expert_stats",
     "moe_rd_sort_workspace_bytes", "moe_rd_sort_tokens", "moe_rd_unsort_tokens", "moe_rd_unsort_tokens_backward",
-    "moe_rd_routing_weights", "moe_rd_routing_weights_backward", "moe_rd_expert_matvec_w4",
+    "moe_rd_routing_weights", "moe_rd_routing_weights_backward", "moe_rd_expert_matvec_w4", "moe_rd_pack_w4",
     "moe_rd_launch_count", "moe_rd_strerror", "moe_rd_last_cuda_error", "moe_rd_version",
 )
 
@@ -141,7 +141,8 @@ def lib() -> ctypes.CDLL:
                 ("moe_rd_unsort_tokens_backward", [i64, i32, i32, i32, ptr, ptr, i64] + [ptr] * 6),
                 ("moe_rd_routing_weights", [i64, i32, i32, i32, i32, f32, f32] + [ptr] * 6),
                 ("moe_rd_routing_weights_backward", [i64, i32, i32, i32, i32, f32, f32] + [ptr] * 7),
-                ("moe_rd_expert_matvec_w4", [i64, i32, i32, i32, i32, i32] + [ptr] * 7)):
+                ("moe_rd_expert_matvec_w4", [i64, i32, i32, i32, i32, i32] + [ptr] * 7),
+                ("moe_rd_pack_w4", [i32, i32, i32, ptr, ptr, ptr])):
             getattr(L, name).argtypes = argtypes
             getattr(L, name).restype = ctypes.c_int
         L.moe_rd_read_status.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(ctypes.c_int32)]

@@ -60,19 +60,23 @@ def pack_w4(q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor]
         if t is not None and t.device != q.device:
             raise ValueError("pack_w4: all tensors must be on one device")
     blocks, chunks = -(-N // 32), -(-K // 128)
-    full = q.new_zeros((E, blocks * 32, chunks * 64))
-    full[:, :N, :half] = q
-    # [E, block, part, output, chunk, word, lane j, byte] -> [E, block, chunk, part, output, j, word, byte]
-    r = full.reshape(E, blocks, 4, 8, chunks, 4, 4, 4).permute(0, 1, 4, 2, 3, 6, 5, 7)
-    packed = torch.empty(r.shape, dtype=torch.uint8, device=q.device)
-    packed[..., 0] = (r[..., 0] & 15) | ((r[..., 1] & 15) << 4)
-    packed[..., 1] = (r[..., 2] & 15) | ((r[..., 3] & 15) << 4)
-    packed[..., 2] = (r[..., 0] >> 4) | (r[..., 1] & 0xF0)
-    packed[..., 3] = (r[..., 2] >> 4) | (r[..., 3] & 0xF0)
+    packed = torch.empty((E, blocks, chunks, 2048), dtype=torch.uint8, device=q.device)
+    if q.is_cuda:
+        call(q.device, _cabi.lib().moe_rd_pack_w4, E, N, K, _ptr(_aligned(q)), _ptr(packed))
+    else:
+        full = q.new_zeros((E, blocks * 32, chunks * 64))
+        full[:, :N, :half] = q
+        # [E, block, part, output, chunk, word, lane j, byte] -> [E, block, chunk, part, output, j, word, byte]
+        r = full.reshape(E, blocks, 4, 8, chunks, 4, 4, 4).permute(0, 1, 4, 2, 3, 6, 5, 7)
+        o = packed.view(r.shape)
+        o[..., 0] = (r[..., 0] & 15) | ((r[..., 1] & 15) << 4)
+        o[..., 1] = (r[..., 2] & 15) | ((r[..., 3] & 15) << 4)
+        o[..., 2] = (r[..., 0] >> 4) | (r[..., 1] & 0xF0)
+        o[..., 3] = (r[..., 2] >> 4) | (r[..., 3] & 0xF0)
     if zeros is not None:
         z = _blocked(zeros)
         zeros = z[..., 0::2] | (z[..., 1::2] << 4)
-    return W4Weights(packed.reshape(E, blocks, chunks, 2048), _blocked(scales), zeros, N, K, group)
+    return W4Weights(packed, _blocked(scales), zeros, N, K, group)
 
 
 def expert_matvec_w4(x: torch.Tensor, weights: W4Weights, offsets: Optional[torch.Tensor] = None, *,

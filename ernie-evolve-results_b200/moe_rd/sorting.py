@@ -30,6 +30,9 @@ class UnsortGradients(NamedTuple):
     weights: Optional[torch.Tensor]  # [T, K] fp32 gradient of the weights
 
 
+_VECTOR = {torch.bfloat16: 8, torch.float16: 8, torch.float32: 4}  # elements in 16 bytes
+
+
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
@@ -37,8 +40,9 @@ def _ptr(t: Optional[torch.Tensor]):
 def check_device(name: str, *tensors: Optional[torch.Tensor]) -> torch.device:
     """The one CUDA device of all the tensors."""
     dev = tensors[0].device
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != dev:
+        if t is not None and t.get_device() != index:
             raise ValueError(f"{name}: all tensors must be on one device, got {dev} and {t.device}")
     if dev.type != "cuda":
         raise RuntimeError(f"moe_rd.{name} has no CPU path: its tensors must be CUDA tensors")
@@ -64,14 +68,13 @@ def spans(*tensors: Optional[torch.Tensor]):
 
 def check_out(name: str, out: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, dev: torch.device, inputs, align: int = 1) -> None:
     """``out`` is a buffer the call may write: of this shape and type, contiguous, apart from the inputs (``spans``)."""
-    if out.shape != shape or out.dtype != dtype or out.device != dev or not out.is_contiguous() or out.requires_grad:
+    if out.shape != shape or out.dtype is not dtype or out.get_device() != dev.index or not out.is_contiguous() or out.requires_grad:
         raise ValueError(f"{name}: out must be a contiguous {dtype} tensor of shape {tuple(shape)} on {dev} that needs no gradient")
     lo = out.data_ptr()
     if lo % align:
         raise ValueError(f"{name}: out must be {align}-byte aligned")
-    hi = lo + out.nbytes
     for begin, end in inputs:
-        if lo < end and begin < hi:
+        if lo < end and begin < lo + out.nbytes:
             raise ValueError(f"{name}: out must not share memory with an input")
 
 
@@ -91,19 +94,21 @@ def _not_while_capturing(name: str, instead: str) -> None:
 
 
 def _check_ids(name: str, ids: torch.Tensor) -> Tuple[int, int]:
-    if ids.dtype != torch.int32:
+    if ids.dtype is not torch.int32:
         raise TypeError(f"{name}: row and expert indices must be int32")
-    if ids.dim() != 2 or ids.shape[1] < 1:
+    shape = ids.shape
+    if len(shape) != 2 or shape[1] < 1:
         raise ValueError(f"{name}: row and expert indices must be [T, K]")
-    return ids.shape[0], ids.shape[1]
+    return shape
 
 
 def _check_rows(name: str, rows: torch.Tensor) -> int:
-    if rows.dtype not in ROW_DTYPE:
+    if rows.dtype not in _VECTOR:
         raise TypeError(f"{name}: rows must be bfloat16, float16 or float32")
-    if rows.dim() < 2 or rows.shape[-1] < 1 or rows.shape[-1] * rows.element_size() % 16:
+    shape = rows.shape
+    if len(shape) < 2 or shape[-1] < 1 or shape[-1] % _VECTOR[rows.dtype]:
         raise ValueError(f"{name}: rows must be [..., H] with H * element size a multiple of 16 bytes")
-    return rows.shape[-1]
+    return shape[-1]
 
 
 def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -198,7 +203,7 @@ def _check_unsort(name, y, inverse_perm, weights, shared):
     if shared is not None:
         if shared.dtype != y.dtype:
             raise TypeError(f"{name}: the [T, H] tensor must have the type of the rows")
-        if shared.dim() < 1 or shared.shape[-1] != H or shared.numel() != T * H:
+        if shared.shape != (T, H) and (shared.dim() < 1 or shared.shape[-1] != H or shared.numel() != T * H):
             raise ValueError(f"{name}: expected a tensor of T = {T} rows of {H}")
     return T, K, H
 

@@ -495,6 +495,13 @@ int moe_rd_expert_matvec_w4(int64_t rows, int32_t N, int32_t K, int32_t E, int32
                             const void* x, const void* weight, const void* scales, const uint16_t* zeros,
                             const int32_t* offsets, void* out, void* stream);
 
+/*
+ * The weight layout of moe_rd_expert_matvec_w4 from q [E,N,K/2] (byte b of an output:
+ * input 2b in the low, 2b+1 in the high four bits): weight [E][B][C][2048 bytes].
+ * K % 32 == 0; both 16-byte aligned.
+ */
+int moe_rd_pack_w4(int32_t E, int32_t N, int32_t K, const uint8_t* q, void* weight, void* stream);
+
 /* Kernels this library launched since it was loaded (all threads). */
 int64_t moe_rd_launch_count(void);
 

@@ -74,6 +74,16 @@ def test_expert_products(E, N, K, group, dtype, zeros, rows, behind):
         assert torch.equal(moe_rd.expert_matvec_w4(x.cuda(), packed), got)
 
 
+@pytest.mark.parametrize("E,N,K", [(1, 1, 32), (3, 45, 160), (2, 64, 1024), (5, 33, 416)])
+def test_weights_laid_out_on_the_gpu_and_on_the_cpu_are_the_same(E, N, K):
+    q, s, z, _ = make(E, N, K, 32, "bf16", True)
+    for a, b in zip(moe_rd.pack_w4(q, s, z), moe_rd.pack_w4(q.cuda(), s.cuda(), z.cuda())):
+        assert torch.equal(a, b.cpu()) if isinstance(a, torch.Tensor) else a == b
+    wide = torch.zeros(E, N, K // 2 + 3, dtype=torch.uint8).cuda()
+    wide[..., 3:] = q.cuda()
+    assert torch.equal(moe_rd.pack_w4(wide[..., 3:], s.cuda(), z.cuda()).packed.cpu(), moe_rd.pack_w4(q, s, z).packed)
+
+
 def test_every_value_and_zero_point_is_exact():
     """One input at a time: the product is the weight itself, for all 16 values and 16 zero points."""
     q = (torch.arange(16).repeat(16, 2) | (torch.arange(16).repeat(16, 2) << 4)).to(torch.uint8)[:, :16]   # K = 32: every value twice

@@ -153,6 +153,11 @@ def test_c_entries_validate_before_any_cuda_call():
     assert mv(ptrs=(0, p, p, None, p, p)) == mv(ptrs=(p, p, p, None, p, 0)) == -1
     assert mv(ptrs=(p + 2, p, p, None, p, p)) == mv(ptrs=(p, p + 8, p, None, p, p)) == mv(ptrs=(p, p, p, None, p, p + 1)) == -4
 
+    def pack(E=1, N=8, K=64, q=p, w=p):
+        return L.moe_rd_pack_w4(E, N, K, q, w, None)
+    assert pack(E=0) == pack(E=257) == pack(N=0) == pack(K=48) == pack(K=0) == -2
+    assert pack(q=0) == pack(w=0) == -1 and pack(q=p + 4) == pack(w=p + 8) == -4
+
 
 def test_capturing_is_refused_where_a_gradient_is_wanted(monkeypatch):
     from moe_rd import sorting
