@@ -17,6 +17,8 @@
 // Leaving the subtraction to the sums (operands 128 + q or 16 + q, and (16 + zero) * sum of x taken off afterwards) saves a
 // quarter of the instructions and was slower: the sums of x cost matrix instructions, and it is their chains that a warp
 // waits for (8 experts x 8192 outputs x 7168 inputs 51.3 against 50.3 us; groups of 32 64.5 against 54.4 us).
+// The copies alone run at 6.7 TB/s (64 experts x 4096 x 7168: 145 us), the kernel at 5.4 (179 us): what bounds it is the
+// integer pipe, 7 instructions for 8 bf16 weights (5 for fp16, 8 % faster).
 //
 // A unit of work is 32 outputs of one expert for up to eight of its rows; its tiles lie one behind the other in memory,
 // and so do the units of an expert.  Only experts that have rows get units: every block lists them from the offsets.  A
@@ -39,7 +41,8 @@ namespace {
 constexpr int kW4Threads = 512;
 constexpr int kW4Warps = kW4Threads / 32;
 // Tiles in flight per warp: 2 KB x 16 warps x 2 is 64 KB an SM, more than a microsecond of its share of the HBM rate.
-// Deeper rings only put off the products: 8 experts x 2048 outputs x 7168 inputs 18.0 us with 2, 19.1 with 3, 19.8 with 4.
+// Deeper rings are slower: 8 experts x 2048 outputs x 7168 inputs, one row each, 18.4 us with 2, 19.0 with 3, 19.7 with 4;
+// 64 experts x 4096 179, 184, 193 us.
 constexpr int kDepth = 2;
 constexpr int kTileBytes = 2048;
 
@@ -222,7 +225,7 @@ __device__ __noinline__ void w4_join(const W4Args& a, const W4Joint& s, int rows
   const unsigned continues = __ballot_sync(kFull, what & kContinues), ends = __ballot_sync(kFull, what & kEnds);
   unsigned begins = __ballot_sync(kFull, what & kBegins);
   for (int k = 0; begins != 0; ++k, begins &= begins - 1) {
-    if ((k & 1) != tid >> 8) continue;
+    if (k % (kW4Threads / 256) != tid >> 8) continue;
     const int w = __ffs(begins) - 1;
     const int last = w + __ffs(ends >> (w + 1));
     const W4Place p = s.place[w];
@@ -239,9 +242,10 @@ template <int DT, int SPAN, bool ZEROS>
 __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
   using Ty = W4Type<DT>;
   using St = W4Stage<SPAN, ZEROS>;
-  extern __shared__ __align__(16) unsigned char s_ring[];  // [warps][kDepth][St::kBytes]
+  extern __shared__ __align__(16) unsigned char s_dynamic[];  // W4Joint, then the rings [warps][kDepth][St::kBytes]
   __shared__ int s_w[kW4Warps], s_u[kW4Warps];
-  __shared__ W4Joint s;
+  W4Joint& s = *reinterpret_cast<W4Joint*>(s_dynamic);
+  unsigned char* s_ring = s_dynamic + sizeof(W4Joint);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, j = lane & 3;
   const Ty ty;
@@ -295,7 +299,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
     first_row = last_row = 0;
   }
   if (tid < kW4Warps) {  // for the call of w4_join that writes nothing
-    s.what[tid] = tid < 2 ? kBegins : kContinues | kEnds;
+    s.what[tid] = tid < kW4Threads / 256 ? kBegins : kContinues | kEnds;
     s.place[tid] = W4Place{0, 0, 0, 0};
   }
   __syncthreads();
@@ -394,11 +398,11 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
     // the rest of this unit, or of the share
     const int stretch = min(t, a.chunks - here.c);
     t -= stretch;
-    // one tile with x in `x`, while the x of the next is fetched into `x_next`
-    const int c_end = here.c + stretch;
-    auto tile = [&](const uint4 (&x)[4], uint4 (&x_next)[4]) {
+#pragma unroll 1
+    for (const int c_end = here.c + stretch; here.c < c_end; ++here.c) {
+      uint4 x[4];
+      w4_load_x(a, xp, here.c, x);
       xp += 256;
-      if (here.c + 1 < c_end) w4_load_x(a, xp, here.c + 1, x_next);
       asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
       __syncwarp();  // the scales of a tile are copied by all lanes
       const unsigned char* st = ring_p + slot;
@@ -422,16 +426,6 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
             return i & 1 ? Ty::second(v) : Ty::first(v);
           },
           [&](int k, int i) { return Ty::zero_operand((zp[k] >> (4 * i)) & 15u); }, acc);
-      ++here.c;
-    };
-    uint4 x0[4], x1[4];
-    w4_load_x(a, xp, here.c, x0);
-#pragma unroll 1
-    while (true) {
-      tile(x0, x1);
-      if (here.c == c_end) break;
-      tile(x1, x0);
-      if (here.c == c_end) break;
     }
     const bool ended = here.c == a.chunks;
     if (began && ended) {
@@ -486,7 +480,8 @@ __global__ void __launch_bounds__(256) pack_w4_kernel(const unsigned char* __res
 
 template <int DT, int SPAN, bool ZEROS>
 cudaError_t launch_w4(const W4Args& a, cudaStream_t s) {
-  constexpr int smem = kW4Warps * kDepth * W4Stage<SPAN, ZEROS>::kBytes;
+  constexpr int smem = sizeof(W4Joint) + kW4Warps * kDepth * W4Stage<SPAN, ZEROS>::kBytes;
+  static_assert(sizeof(W4Joint) % 16 == 0, "the rings are 16-byte aligned");
   static std::atomic<uint64_t> set{0};  // devices whose kernel has its shared memory; setting it twice does no harm
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
