@@ -17,8 +17,8 @@
 // Leaving the subtraction to the sums (operands 128 + q or 16 + q, and (16 + zero) * sum of x taken off afterwards) saves a
 // quarter of the instructions and was slower: the sums of x cost matrix instructions, and it is their chains that a warp
 // waits for (8 experts x 8192 outputs x 7168 inputs 51.3 against 50.3 us; groups of 32 64.5 against 54.4 us).
-// The copies alone run at 6.7 TB/s (64 experts x 4096 x 7168: 145 us), the kernel at 5.4 (179 us): what bounds it is the
-// integer pipe, 7 instructions for 8 bf16 weights (5 for fp16, 8 % faster).
+// The copies alone run at 6.7 TB/s (64 experts x 4096 x 7168: 145 us), the kernel at 5.5 (175 us): what bounds it is the
+// integer pipe, 7 instructions for 8 bf16 weights (5 for fp16, 6 % faster).
 //
 // A unit of work is 32 outputs of one expert for up to eight of its rows; its tiles lie one behind the other in memory,
 // and so do the units of an expert.  Only experts that have rows get units: every block lists them from the offsets.  A
@@ -40,10 +40,10 @@ namespace {
 
 constexpr int kW4Threads = 512;
 constexpr int kW4Warps = kW4Threads / 32;
-// Tiles in flight per warp: 2 KB x 16 warps x 2 is 64 KB an SM, more than a microsecond of its share of the HBM rate.
-// Deeper rings are slower: 8 experts x 2048 outputs x 7168 inputs, one row each, 18.4 us with 2, 19.0 with 3, 19.7 with 4;
-// 64 experts x 4096 179, 184, 193 us.
-constexpr int kDepth = 2;
+// Tiles in flight per warp while another is being multiplied: 2 KB x 16 warps is 32 KB an SM, most of a microsecond of its
+// share of the HBM rate.  Deeper rings are slower: 64 experts x 4096 outputs x 7168 inputs, one row each, 175 us with 1, 181
+// with 2; 8 experts x 2048 outputs 17.8, 18.4 us.
+constexpr int kDepth = 1;
 constexpr int kTileBytes = 2048;
 
 struct W4Args {
@@ -176,15 +176,16 @@ __device__ __forceinline__ void w4_tile(const W4Type<DT>& ty, const uint4 (&w)[4
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
-__device__ __forceinline__ void copy8(uint32_t to, const void* from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+// 8 bytes, of which the first `bytes` (0 or 8) are read and the rest become zero
+__device__ __forceinline__ void copy8(uint32_t to, const void* from, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copy4(uint32_t to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
 
-__device__ __forceinline__ uint32_t w4_group(const W4Args& a, uint32_t b) {  // of block b of 32 inputs
-  return min(a.group_magic != 0 ? __umulhi(b, a.group_magic) : b, (uint32_t)a.G - 1);
+__device__ __forceinline__ uint32_t w4_group(const W4Args& a, uint32_t b) {  // of block b of 32 inputs; G or more: padding
+  return a.group_magic != 0 ? __umulhi(b, a.group_magic) : b;
 }
 
 __device__ __forceinline__ void w4_load_x(const W4Args& a, const unsigned char* xp, int c, uint4 (&x)[4]) {
@@ -258,9 +259,9 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
   } else {
     if (tid < a.E) {
       lo = __ldg(a.offsets + tid);
-      n = __ldg(a.offsets + tid + 1) - lo;
+      const int hi = __ldg(a.offsets + tid + 1);
       // offsets that decrease or leave the rows are nobody's: every row becomes zero
-      if (lo < 0 || n < 0 || n > (int)a.rows - lo) n = INT_MIN;
+      n = lo < 0 || hi < lo || hi > (int)a.rows ? INT_MIN : hi - lo;
     }
     first_row = __ldg(a.offsets);
     last_row = __ldg(a.offsets + a.E);
@@ -352,8 +353,9 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) copy16(to + i * 512 + lane * 16, next_w + i * 512);
       if (j < St::kParts) {
-        const uint32_t gr = w4_group(a, 4 * next.c + SPAN * j);
-        copy8(to + St::kScales + (j * 8 + g) * 8, next_s + (size_t)gr * 64);
+        // a group of padding alone has scale zero (its products are zero, and zero times an infinite scale is no number)
+        const uint32_t of = w4_group(a, 4 * next.c + SPAN * j), gr = min(of, (uint32_t)a.G - 1);
+        copy8(to + St::kScales + (j * 8 + g) * 8, next_s + (size_t)gr * 64, of == gr ? 8u : 0u);
         if (ZEROS && g < 4) copy4(to + St::kZeros + j * 16 + g * 4, next_z + (size_t)gr * 16);
       }
       next_w += kTileBytes;
@@ -398,11 +400,11 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
     // the rest of this unit, or of the share
     const int stretch = min(t, a.chunks - here.c);
     t -= stretch;
-#pragma unroll 1
-    for (const int c_end = here.c + stretch; here.c < c_end; ++here.c) {
-      uint4 x[4];
-      w4_load_x(a, xp, here.c, x);
+    // one tile with its inputs in `x`, while those of the next are fetched into `x_next`
+    const int c_end = here.c + stretch;
+    auto tile = [&](const uint4 (&x)[4], uint4 (&x_next)[4]) {
       xp += 256;
+      if (here.c + 1 < c_end) w4_load_x(a, xp, here.c + 1, x_next);
       asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
       __syncwarp();  // the scales of a tile are copied by all lanes
       const unsigned char* st = ring_p + slot;
@@ -426,6 +428,16 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
             return i & 1 ? Ty::second(v) : Ty::first(v);
           },
           [&](int k, int i) { return Ty::zero_operand((zp[k] >> (4 * i)) & 15u); }, acc);
+      ++here.c;
+    };
+    uint4 x0[4], x1[4];
+    w4_load_x(a, xp, here.c, x0);
+#pragma unroll 1
+    while (true) {
+      tile(x0, x1);
+      if (here.c == c_end) break;
+      tile(x1, x0);
+      if (here.c == c_end) break;
     }
     const bool ended = here.c == a.chunks;
     if (began && ended) {

@@ -132,12 +132,15 @@ __global__ void __launch_bounds__(kRwThreads, LOGITS <= 16 ? 4 : 3) routing_weig
       dsk = __fmul_rn(__fmul_rn(q, r), r);
     }
     const float u = valid ? __fadd_rn(sk, kb) : 0.0f;
-    float total = 0.0f;
-    if (a.renorm) total = token_sum<W>(u);
+    float total = 1.0f, divisor = 1.0f;
+    if (a.renorm) {
+      total = token_sum<W>(u);
+      divisor = total < a.norm_min ? a.norm_min : total;  // a sum that is no number stays one
+    }
 
     if (!BACKWARD) {
       if (live && slot < a.K) {
-        const float w = a.renorm ? __fdiv_rn(u, fmaxf(total, a.norm_min)) : u;
+        const float w = a.renorm ? __fdiv_rn(u, divisor) : u;
         a.out[(size_t)t * a.K + slot] = valid ? __fmul_rn(w, a.routed_scale) : 0.0f;
       }
       continue;
@@ -146,7 +149,7 @@ __global__ void __launch_bounds__(kRwThreads, LOGITS <= 16 ? 4 : 3) routing_weig
     float h = __fmul_rn(a.routed_scale, gw);
     bool flat = !SOFTMAX;  // D = 0: no gradient but that of the chosen experts
     if (a.renorm) {
-      const bool moving = total >= a.norm_min;
+      const bool moving = !(total < a.norm_min);
       const float part = __fdiv_rn(u, total);
       float diff = 0.0f;
       for (int k = 0; k < a.K; ++k) {
@@ -157,7 +160,7 @@ __global__ void __launch_bounds__(kRwThreads, LOGITS <= 16 ? 4 : 3) routing_weig
         h = diff;
         if (a.select_bias == nullptr) flat = true;
       }
-      h = valid ? __fdiv_rn(h, moving ? total : a.norm_min) : 0.0f;
+      h = valid ? __fdiv_rn(h, divisor) : 0.0f;
     }
     // slots with the same expert are added by the first of them, in slot order
     const unsigned group = W == 32 ? kFull : (((1u << W) - 1u) << (lane & ~(W - 1)));

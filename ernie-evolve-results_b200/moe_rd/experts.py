@@ -8,7 +8,7 @@ import torch
 
 from . import _cabi
 from ._cabi import ROW_DTYPE
-from .sorting import _aligned, _check_offsets, _ptr, call, check_device, check_out, spans, wants_grad
+from .sorting import _aligned, _check_offsets, _ptr, call, check_device, check_out, spans, wants_grad, written
 
 
 class W4Weights(NamedTuple):
@@ -115,10 +115,11 @@ def expert_matvec_w4(x: torch.Tensor, weights: W4Weights, offsets: Optional[torc
     dev = check_device("expert_matvec_w4", x, packed, scales, zeros, offsets)
     x2 = _aligned(x)
     R = x.shape[0]
-    if out is None:
-        out = torch.empty((R, N), dtype=x.dtype, device=dev)
-    else:
+    result = torch.empty((R, N), dtype=x.dtype, device=dev) if out is None else out
+    if out is not None:
         check_out("expert_matvec_w4", out, (R, N), x.dtype, dev, spans(x2, packed, scales, zeros, offsets))
     call(dev, _cabi.lib().moe_rd_expert_matvec_w4, R, N, K, E, group, ROW_DTYPE[x.dtype], _ptr(x2), _ptr(packed), _ptr(scales),
-         _ptr(zeros), _ptr(offsets), _ptr(out))
-    return out
+         _ptr(zeros), _ptr(offsets), _ptr(result))
+    if out is not None:
+        written(out)
+    return result

@@ -78,6 +78,12 @@ def check_out(name: str, out: torch.Tensor, shape: Tuple[int, ...], dtype: torch
             raise ValueError(f"{name}: out must not share memory with an input")
 
 
+def written(*out: Optional[torch.Tensor]) -> None:
+    """Tell autograd that these buffers of the caller have been overwritten: a graph that saved one of them then raises in
+    its backward pass instead of computing with the new contents."""
+    torch.autograd.graph.increment_version([t for t in out if t is not None])
+
+
 def wants_grad(*tensors: Optional[torch.Tensor]) -> bool:
     if torch.is_grad_enabled():
         for t in tensors:
@@ -130,8 +136,9 @@ def _sort(x, expert_ids, num_experts, capacity, out):
     R = min(T * K, E * capacity) if capacity else T * K
     if out is None:
         offsets, inv, row_token, counts = torch.empty(2 * E + 1 + T * K + R, dtype=torch.int32, device=dev).split((E + 1, T * K, R, E))
-        out = SortedTokens(torch.empty((R, H), dtype=x.dtype, device=dev), offsets, inv.view(T, K), row_token, counts)
+        result = SortedTokens(torch.empty((R, H), dtype=x.dtype, device=dev), offsets, inv.view(T, K), row_token, counts)
     else:
+        result = out
         given = spans(x2, ids)
         check_out("sort_tokens", out.rows, (R, H), x.dtype, dev, given, 16)
         check_out("sort_tokens", out.offsets, (E + 1,), torch.int32, dev, given)
@@ -140,9 +147,11 @@ def _sort(x, expert_ids, num_experts, capacity, out):
         check_out("sort_tokens", out.counts, (E,), torch.int32, dev, given)
     ws_bytes = _cabi.sort_workspace_bytes(T, H, E, K, ROW_DTYPE[x.dtype])
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-    call(dev, _cabi.lib().moe_rd_sort_tokens, T, H, E, K, ROW_DTYPE[x.dtype], capacity, R, _ptr(x2), _ptr(ids), _ptr(out.rows),
-         _ptr(out.offsets), _ptr(out.inverse_perm), _ptr(out.row_token), _ptr(out.counts), _ptr(ws), ws_bytes)
-    return out
+    call(dev, _cabi.lib().moe_rd_sort_tokens, T, H, E, K, ROW_DTYPE[x.dtype], capacity, R, _ptr(x2), _ptr(ids), _ptr(result.rows),
+         _ptr(result.offsets), _ptr(result.inverse_perm), _ptr(result.row_token), _ptr(result.counts), _ptr(ws), ws_bytes)
+    if out is not None:
+        written(*out)
+    return result
 
 
 class _SortTokens(torch.autograd.Function):
@@ -216,13 +225,14 @@ def _unsort(y, inverse_perm, weights, shared, out):
     inv = inverse_perm.contiguous()
     w = None if weights is None else weights.contiguous()
     sh = None if shared is None else _aligned(shared if shared.dim() == 2 else shared.reshape(T, H))
-    if out is None:
-        out = torch.empty((T, H), dtype=y.dtype, device=dev)
-    else:
+    result = torch.empty((T, H), dtype=y.dtype, device=dev) if out is None else out
+    if out is not None:
         check_out("unsort_tokens", out, (T, H), y.dtype, dev, spans(y2, inv, w, sh), 16)
     call(dev, _cabi.lib().moe_rd_unsort_tokens, T, H, K, ROW_DTYPE[y.dtype], _ptr(y2), y2.shape[0], _ptr(inv), _ptr(w),
-         _ptr(sh), _ptr(out))
-    return out
+         _ptr(sh), _ptr(result))
+    if out is not None:
+        written(out)
+    return result
 
 
 class _UnsortTokens(torch.autograd.Function):
@@ -291,9 +301,10 @@ def _unsort_backward(grad_out, y, y_shape, inverse_perm, weights, offsets, need_
     inv = inverse_perm.contiguous()
     w = None if weights is None else weights.contiguous()
     if out is None:
-        out = UnsortGradients(torch.empty(y_shape, dtype=g.dtype, device=dev) if need_y else None,
-                              torch.empty((T, K), dtype=torch.float32, device=dev) if need_w else None)
+        result = UnsortGradients(torch.empty(y_shape, dtype=g.dtype, device=dev) if need_y else None,
+                                 torch.empty((T, K), dtype=torch.float32, device=dev) if need_w else None)
     else:
+        result = out
         if (out.rows is not None) != need_y or (out.weights is not None) != need_w:
             raise ValueError("unsort_tokens_backward: out must hold the gradients that are asked for")
         given = spans(g, y2, inv, w, offsets)
@@ -303,8 +314,10 @@ def _unsort_backward(grad_out, y, y_shape, inverse_perm, weights, offsets, need_
             check_out("unsort_tokens_backward", out.weights, (T, K), torch.float32, dev, given)
     n_rows = None if offsets is None else offsets.data_ptr() + 4 * (offsets.numel() - 1)
     call(dev, _cabi.lib().moe_rd_unsort_tokens_backward, T, H, K, ROW_DTYPE[g.dtype], _ptr(g), _ptr(y2), R, _ptr(inv), _ptr(w),
-         n_rows, _ptr(out.rows), _ptr(out.weights))
-    return out
+         n_rows, _ptr(result.rows), _ptr(result.weights))
+    if out is not None:
+        written(*out)
+    return result
 
 
 def unsort_tokens_backward(grad_out: torch.Tensor, y: torch.Tensor, inverse_perm: torch.Tensor,
@@ -388,11 +401,14 @@ def routing_weights(logits: torch.Tensor, expert_ids: torch.Tensor, bias: Option
         _not_while_capturing("routing_weights", "routing_weights on detached logits and routing_weights_backward")
         return _RoutingWeights.apply(logits, expert_ids, bias, config)
     if out is None:
-        out = torch.empty(expert_ids.shape, dtype=torch.float32, device=dev)
+        result = torch.empty(expert_ids.shape, dtype=torch.float32, device=dev)
     else:
+        result = out
         check_out("routing_weights", out, expert_ids.shape, torch.float32, dev, spans(logits, expert_ids, bias))
-    _weights_call(_cabi.lib().moe_rd_routing_weights, logits, expert_ids, bias, *config, out)
-    return out
+    _weights_call(_cabi.lib().moe_rd_routing_weights, logits, expert_ids, bias, *config, result)
+    if out is not None:
+        written(out)
+    return result
 
 
 def routing_weights_backward(grad_weights: torch.Tensor, logits: torch.Tensor, expert_ids: torch.Tensor,
@@ -408,9 +424,12 @@ def routing_weights_backward(grad_weights: torch.Tensor, logits: torch.Tensor, e
     dev = check_device("routing_weights_backward", logits, grad_weights, expert_ids, bias)
     grad = grad_weights.contiguous()
     if out is None:
-        out = torch.empty(logits.shape, dtype=torch.float32, device=dev)
+        result = torch.empty(logits.shape, dtype=torch.float32, device=dev)
     else:
+        result = out
         check_out("routing_weights_backward", out, logits.shape, torch.float32, dev, spans(logits, expert_ids, bias, grad))
     _weights_call(_cabi.lib().moe_rd_routing_weights_backward, logits, expert_ids, bias, bias_mode, score_fn, renorm, routed_scale,
-                  norm_min, grad, out)
-    return out
+                  norm_min, grad, result)
+    if out is not None:
+        written(out)
+    return result

@@ -117,6 +117,34 @@ def test_nan_and_inf_reach_only_their_rows_and_outputs(dtype):
     check(x[rows], w[:, keep], [0, 4], got[rows][:, keep], dtype, 1152)
 
 
+@pytest.mark.parametrize("K,group", [(160, 32), (192, 64), (288, 96)])
+def test_an_infinite_scale_next_to_padded_inputs(K, group):
+    """The last group's scale is infinite and the last tile has inputs that do not exist."""
+    q, s, z, w = make(1, 9, K, group, "fp16", False)
+    s[0, 4, -1] = float("inf")
+    keep = torch.arange(9) != 4
+    x = torch.zeros(2, K, dtype=torch.float16)
+    x[:, -1] = 1.0
+    got = moe_rd.expert_matvec_w4(x.cuda(), moe_rd.pack_w4(q.cuda(), s.cuda())).cpu()
+    assert not torch.isfinite(got[:, 4]).any()      # infinite weights times inputs of zero and one
+    check(x, w[:, keep], [0, 2], got[:, keep], "fp16", K)
+    # infinite weights of one sign times inputs of one sign: an infinity, and the inputs that do not exist do not spoil it
+    q[0, 4] = 0xFF
+    got = moe_rd.expert_matvec_w4(torch.ones_like(x).cuda(), moe_rd.pack_w4(q.cuda(), s.cuda())).cpu()
+    assert (got[:, 4] == float("inf")).all() and torch.isfinite(got[:, keep]).all()
+
+
+def test_offsets_that_make_no_sense_give_zeros():
+    q, s, _, _ = make(4, 40, 128, 32, "bf16", False)
+    p = moe_rd.pack_w4(q.cuda(), s.cuda())
+    x = torch.randn(10, 128).to(torch.bfloat16).cuda()
+    for off in ([0, 5, 3, 8, 10], [0, 2, 4, 6, 11], [-1, 2, 4, 6, 10], [0, 2 ** 31 - 1, 4, 6, 10], [0, 1, 2, 2, -2 ** 31]):
+        got = moe_rd.expert_matvec_w4(x, p, torch.tensor(off, dtype=torch.int32).cuda())
+        assert (got == 0).all()
+    got = moe_rd.expert_matvec_w4(x, p, torch.tensor([3, 4, 4, 6, 7], dtype=torch.int32).cuda())
+    assert (got[:3] == 0).all() and (got[7:] == 0).all() and (got[3:7] != 0).any(1).all()
+
+
 def test_the_decode_step_of_a_layer():
     """route_dispatch, the two 4-bit products of a gated expert layer, and combine, for one token and for several."""
     E, H, I, K = 16, 256, 128, 4

@@ -143,6 +143,17 @@ def test_masked_and_extreme_logits():
                 assert ((got_g[t].double() - want_g[t]).abs() <= 2e-4 * want_g[t].abs().max() + 1e-37).all()
 
 
+def test_a_logit_that_is_no_number_reaches_all_of_its_token():
+    logits = torch.randn(4, 12)
+    logits[1, 5] = float("nan")
+    ids = torch.tensor([[0, 1], [5, 2], [3, 4], [5, 6]], dtype=torch.int32)
+    for score_fn in ("softmax", "sigmoid"):
+        w = moe_rd.routing_weights(logits.cuda(), ids.cuda(), score_fn=score_fn).cpu()
+        g = moe_rd.routing_weights_backward(torch.ones(4, 2).cuda(), logits.cuda(), ids.cuda(), score_fn=score_fn).cpu()
+        assert torch.isnan(w[1]).all() and torch.isnan(g[1, ids[1].long()]).all()
+        assert torch.isfinite(w[[0, 2, 3]]).all() and torch.isfinite(g[[0, 2, 3]]).all()
+
+
 def test_sizes_of_nothing_and_graph():
     e = moe_rd.routing_weights(torch.zeros(0, 8).cuda(), torch.zeros(0, 2, dtype=torch.int32).cuda())
     assert e.shape == (0, 2)

@@ -378,3 +378,40 @@ def test_autograd_is_refused_while_capturing():
             with torch.cuda.graph(graph):
                 fn()
     assert torch.equal(moe_rd.sort_tokens(x, ids, 4).inverse_perm, inv)
+
+
+def test_a_buffer_that_backward_needs_cannot_be_reused_unseen():
+    x = torch.randn(50, 64, device="cuda", requires_grad=True)
+    ids = ids_of(50, 2, 8, "random").cuda()
+    s = moe_rd.sort_tokens(x, ids, 8)
+    out = moe_rd.unsort_tokens(s.rows, s.inverse_perm, offsets=s.offsets)
+    moe_rd.sort_tokens(x.detach(), ids.flip(0), 8, out=moe_rd.SortedTokens(torch.empty_like(s.rows), *s[1:]))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    y = torch.randn(100, 64, device="cuda", requires_grad=True)
+    w = torch.rand(50, 2, device="cuda", requires_grad=True)
+    out = moe_rd.unsort_tokens(y, s.inverse_perm, w)
+    moe_rd.routing_weights(torch.randn(50, 8, device="cuda"), ids, out=w.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+def test_out_is_checked():
+    x = torch.randn(20, 64, device="cuda")
+    ids = ids_of(20, 2, 8, "random").cuda()
+    s = moe_rd.sort_tokens(x, ids, 8)
+    for bad in (s._replace(rows=s.rows[:39]), s._replace(rows=s.rows.half()), s._replace(rows=s.rows.cpu()), s._replace(offsets=ids.view(-1)[:9]),
+                s._replace(counts=s.counts.long()), s._replace(rows=torch.empty(64, 40, device="cuda").t()),
+                s._replace(rows=torch.empty(40 * 64 + 1, device="cuda")[1:].view(40, 64))):
+        with pytest.raises(ValueError, match="out must"):
+            moe_rd.sort_tokens(x, ids, 8, out=bad)
+    for bad in (x[:19], x.double(), s.rows[:20], torch.empty(20, 64, device="cuda", requires_grad=True)):
+        with pytest.raises(ValueError, match="out must"):
+            moe_rd.unsort_tokens(s.rows, s.inverse_perm, out=bad)
+    leaf = x.clone().requires_grad_()
+    with pytest.raises(ValueError, match="out cannot"):
+        moe_rd.sort_tokens(leaf, ids, 8, out=s)
+    with pytest.raises(ValueError, match="one device"):
+        moe_rd.sort_tokens(x, ids.cpu(), 8)
+    with pytest.raises(moe_rd.MoeRdError):
+        moe_rd.sort_tokens(x, ids, 257)
