@@ -8,7 +8,7 @@ import torch
 
 from . import _cabi
 from ._cabi import ROW_DTYPE
-from .sorting import _aligned, _check_offsets, _ptr, call, check_device, check_out, spans, wants_grad, written
+from .sorting import call, check_offsets, check_out, dense, device_index, wants_grad, written
 
 
 class W4Weights(NamedTuple):
@@ -62,7 +62,8 @@ def pack_w4(q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor]
     blocks, chunks = -(-N // 32), -(-K // 128)
     packed = torch.empty((E, blocks, chunks, 2048), dtype=torch.uint8, device=q.device)
     if q.is_cuda:
-        call(q.device, _cabi.lib().moe_rd_pack_w4, E, N, K, _ptr(_aligned(q)), _ptr(packed))
+        q, q_at = dense(q)
+        call(q.get_device(), _cabi.lib().moe_rd_pack_w4, E, N, K, q_at, packed.data_ptr())
     else:
         full = q.new_zeros((E, blocks * 32, chunks * 64))
         full[:, :N, :half] = q
@@ -92,34 +93,47 @@ def expert_matvec_w4(x: torch.Tensor, weights: W4Weights, offsets: Optional[torc
     """
     if not isinstance(weights, W4Weights):
         raise TypeError("expert_matvec_w4: weights must come from pack_w4")
-    if x.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError("expert_matvec_w4: rows must be bfloat16 or float16")
-    if weights.scales.dtype != x.dtype:
-        raise TypeError("expert_matvec_w4: rows and scales must have one type")
     packed, scales, zeros, N, K, group = weights
-    E, blocks, chunks = packed.shape[:3]
+    dtype = x.dtype
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise TypeError("expert_matvec_w4: rows must be bfloat16 or float16")
+    if scales.dtype is not dtype:
+        raise TypeError("expert_matvec_w4: rows and scales must have one type")
+    E, blocks = packed.shape[0], -(-N // 32)
     G = K // group
     if x.dim() != 2 or x.shape[1] != K:
         raise ValueError(f"expert_matvec_w4: rows must be [R, {K}]")
-    if (packed.shape != (E, -(-N // 32), -(-K // 128), 2048) or packed.dtype != torch.uint8 or not packed.is_contiguous()
+    if (packed.shape != (E, blocks, -(-K // 128), 2048) or packed.dtype is not torch.uint8 or not packed.is_contiguous()
             or scales.shape != (E, blocks, G, 8, 4) or not scales.is_contiguous()
-            or (zeros is not None and (zeros.shape != (E, blocks, G, 8, 2) or zeros.dtype != torch.uint8 or not zeros.is_contiguous()))):
+            or (zeros is not None and (zeros.shape != (E, blocks, G, 8, 2) or zeros.dtype is not torch.uint8 or not zeros.is_contiguous()))):
         raise ValueError("expert_matvec_w4: weights are not as pack_w4 returns them")
-    _check_offsets("expert_matvec_w4", offsets)
-    if offsets is None and E != 1:
-        raise ValueError("expert_matvec_w4: offsets are needed where there is more than one expert")
-    if offsets is not None and offsets.numel() != E + 1:
-        raise ValueError(f"expert_matvec_w4: offsets must have {E + 1} elements")
+    if offsets is None:
+        if E != 1:
+            raise ValueError("expert_matvec_w4: offsets are needed where there is more than one expert")
+    else:
+        check_offsets("expert_matvec_w4", offsets)
+        if offsets.numel() != E + 1:
+            raise ValueError(f"expert_matvec_w4: offsets must have {E + 1} elements")
     if wants_grad(x, scales):
         raise RuntimeError("expert_matvec_w4 is for inference and has no gradient: pass detached rows")
-    dev = check_device("expert_matvec_w4", x, packed, scales, zeros, offsets)
-    x2 = _aligned(x)
+    index = device_index("expert_matvec_w4", x, packed, scales, zeros, offsets)
+    x, x_at = dense(x)
     R = x.shape[0]
-    result = torch.empty((R, N), dtype=x.dtype, device=dev) if out is None else out
-    if out is not None:
-        check_out("expert_matvec_w4", out, (R, N), x.dtype, dev, spans(x2, packed, scales, zeros, offsets))
-    call(dev, _cabi.lib().moe_rd_expert_matvec_w4, R, N, K, E, group, ROW_DTYPE[x.dtype], _ptr(x2), _ptr(packed), _ptr(scales),
-         _ptr(zeros), _ptr(offsets), _ptr(result))
+    weights_at, scales_at = packed.data_ptr(), scales.data_ptr()
+    zeros_at = None if zeros is None else zeros.data_ptr()
+    offsets_at = None if offsets is None else offsets.data_ptr()
+    if out is None:
+        result = torch.empty((R, N), dtype=dtype, device=x.device)
+        at = result.data_ptr()
+    else:
+        result = out
+        given = [(x_at, x.nbytes), (weights_at, packed.nbytes), (scales_at, scales.nbytes)]
+        if zeros is not None:
+            given.append((zeros_at, zeros.nbytes))
+        if offsets is not None:
+            given.append((offsets_at, 4 * E + 4))
+        at = check_out("expert_matvec_w4", out, (R, N), dtype, index, given)
+    call(index, _cabi.lib().moe_rd_expert_matvec_w4, R, N, K, E, group, ROW_DTYPE[dtype], x_at, weights_at, scales_at, zeros_at, offsets_at, at)
     if out is not None:
         written(out)
     return result

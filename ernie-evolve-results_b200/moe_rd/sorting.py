@@ -33,49 +33,52 @@ class UnsortGradients(NamedTuple):
 _VECTOR = {torch.bfloat16: 8, torch.float16: 8, torch.float32: 4}  # elements in 16 bytes
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
-
-
-def check_device(name: str, *tensors: Optional[torch.Tensor]) -> torch.device:
-    """The one CUDA device of all the tensors."""
-    dev = tensors[0].device
-    index = tensors[0].get_device()
-    for t in tensors:
+def device_index(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """The index of the one CUDA device of all the tensors."""
+    index = first.get_device()
+    for t in others:
         if t is not None and t.get_device() != index:
-            raise ValueError(f"{name}: all tensors must be on one device, got {dev} and {t.device}")
-    if dev.type != "cuda":
+            raise ValueError(f"{name}: all tensors must be on one device, got {first.device} and {t.device}")
+    if index < 0 or not first.is_cuda:
         raise RuntimeError(f"moe_rd.{name} has no CPU path: its tensors must be CUDA tensors")
-    return dev
+    return index
 
 
-def call(dev: torch.device, entry, *args) -> None:
-    """Enqueue a C entry point on the current stream of ``dev``."""
-    index = dev.index
+def call(index: int, entry, *args) -> None:
+    """Enqueue a C entry point on the current stream of CUDA device ``index``."""
     if index == torch.cuda.current_device():
         code = entry(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(index):
             code = entry(*args, torch._C._cuda_getCurrentRawStream(index))
     if code:
         _cabi.check(code)
 
 
-def spans(*tensors: Optional[torch.Tensor]):
-    """The address ranges of dense tensors."""
-    return [(p, p + t.nbytes) for t in tensors if t is not None and (p := t.data_ptr())]
+def dense(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """The tensor, or a copy of it, contiguous and 16-byte aligned (a view may start anywhere), and its address."""
+    if not t.is_contiguous():
+        t = t.contiguous()
+    at = t.data_ptr()
+    if at & 15:
+        t = t.clone()
+        at = t.data_ptr()
+    return t, at
 
 
-def check_out(name: str, out: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, dev: torch.device, inputs, align: int = 1) -> None:
-    """``out`` is a buffer the call may write: of this shape and type, contiguous, apart from the inputs (``spans``)."""
-    if out.shape != shape or out.dtype is not dtype or out.get_device() != dev.index or not out.is_contiguous() or out.requires_grad:
-        raise ValueError(f"{name}: out must be a contiguous {dtype} tensor of shape {tuple(shape)} on {dev} that needs no gradient")
+def check_out(name: str, out: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, index: int, inputs, align: int = 1) -> int:
+    """``out`` is a buffer the call may write: of this shape and type, contiguous, apart from the inputs ((address, bytes)
+    each).  Returns its address."""
+    if out.shape != shape or out.dtype is not dtype or out.get_device() != index or not out.is_contiguous() or out.requires_grad:
+        raise ValueError(f"{name}: out must be a contiguous {dtype} tensor of shape {tuple(shape)} on cuda:{index} that needs no gradient")
     lo = out.data_ptr()
     if lo % align:
         raise ValueError(f"{name}: out must be {align}-byte aligned")
-    for begin, end in inputs:
-        if lo < end and begin < lo + out.nbytes:
+    hi = lo + out.nbytes
+    for at, nbytes in inputs:
+        if lo < at + nbytes and at < hi:
             raise ValueError(f"{name}: out must not share memory with an input")
+    return lo
 
 
 def written(*out: Optional[torch.Tensor]) -> None:
@@ -117,38 +120,31 @@ def _check_rows(name: str, rows: torch.Tensor) -> int:
     return shape[-1]
 
 
-def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    """Dense and 16-byte aligned (a view may start anywhere)."""
-    if t is None:
-        return None
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
 # --- sort ------------------------------------------------------------------------------------------------------------
-def _sort(x, expert_ids, num_experts, capacity, out):
+def _sort(index, x, expert_ids, num_experts, capacity, out):
     H = x.shape[-1]
     T, K = expert_ids.shape
     E = num_experts
-    dev = x.device
-    x2 = _aligned(x if x.dim() == 2 else x.reshape(T, H))
-    ids = expert_ids.contiguous()
+    x, x_at = dense(x if x.dim() == 2 else x.reshape(T, H))
+    ids, ids_at = dense(expert_ids)
     R = min(T * K, E * capacity) if capacity else T * K
+    dtype = x.dtype
+    code = ROW_DTYPE[dtype]
     if out is None:
-        offsets, inv, row_token, counts = torch.empty(2 * E + 1 + T * K + R, dtype=torch.int32, device=dev).split((E + 1, T * K, R, E))
-        result = SortedTokens(torch.empty((R, H), dtype=x.dtype, device=dev), offsets, inv.view(T, K), row_token, counts)
+        ints = torch.empty(2 * E + 1 + T * K + R, dtype=torch.int32, device=x.device)
+        offsets, inv, row_token, counts = ints.split((E + 1, T * K, R, E))
+        result = SortedTokens(torch.empty((R, H), dtype=dtype, device=x.device), offsets, inv.view(T, K), row_token, counts)
+        at = [t.data_ptr() for t in result]
     else:
         result = out
-        given = spans(x2, ids)
-        check_out("sort_tokens", out.rows, (R, H), x.dtype, dev, given, 16)
-        check_out("sort_tokens", out.offsets, (E + 1,), torch.int32, dev, given)
-        check_out("sort_tokens", out.inverse_perm, (T, K), torch.int32, dev, given)
-        check_out("sort_tokens", out.row_token, (R,), torch.int32, dev, given)
-        check_out("sort_tokens", out.counts, (E,), torch.int32, dev, given)
-    ws_bytes = _cabi.sort_workspace_bytes(T, H, E, K, ROW_DTYPE[x.dtype])
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-    call(dev, _cabi.lib().moe_rd_sort_tokens, T, H, E, K, ROW_DTYPE[x.dtype], capacity, R, _ptr(x2), _ptr(ids), _ptr(result.rows),
-         _ptr(result.offsets), _ptr(result.inverse_perm), _ptr(result.row_token), _ptr(result.counts), _ptr(ws), ws_bytes)
+        i32 = torch.int32
+        given = ((x_at, x.nbytes), (ids_at, 4 * T * K))
+        at = (check_out("sort_tokens", out.rows, (R, H), dtype, index, given, 16), check_out("sort_tokens", out.offsets, (E + 1,), i32, index, given),
+              check_out("sort_tokens", out.inverse_perm, (T, K), i32, index, given), check_out("sort_tokens", out.row_token, (R,), i32, index, given),
+              check_out("sort_tokens", out.counts, (E,), i32, index, given))
+    ws_bytes = _cabi.sort_workspace_bytes(T, H, E, K, code)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
+    call(index, _cabi.lib().moe_rd_sort_tokens, T, H, E, K, code, capacity, R, x_at, ids_at, *at, ws.data_ptr() if ws_bytes else None, ws_bytes)
     if out is not None:
         written(*out)
     return result
@@ -157,7 +153,7 @@ def _sort(x, expert_ids, num_experts, capacity, out):
 class _SortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, expert_ids, num_experts, capacity):
-        out = _sort(x, expert_ids, num_experts, capacity, None)
+        out = _sort(x.get_device(), x, expert_ids, num_experts, capacity, None)
         ctx.save_for_backward(out.inverse_perm)
         ctx.shape = x.shape
         ctx.mark_non_differentiable(*out[1:])
@@ -168,7 +164,7 @@ class _SortTokens(torch.autograd.Function):
     def backward(ctx, grad_rows, *_):
         _not_while_capturing("sort_tokens", "sort_tokens on detached tensors and unsort_tokens for its gradient")
         (inverse_perm,) = ctx.saved_tensors
-        return _unsort(grad_rows, inverse_perm, None, None, None).reshape(ctx.shape), None, None, None
+        return _unsort(grad_rows.get_device(), grad_rows, inverse_perm, None, None, None).reshape(ctx.shape), None, None, None
 
 
 def sort_tokens(x: torch.Tensor, expert_ids: torch.Tensor, num_experts: int, *, capacity: int = 0,
@@ -191,9 +187,9 @@ def sort_tokens(x: torch.Tensor, expert_ids: torch.Tensor, num_experts: int, *, 
     if num_experts < 1 or capacity < 0:
         raise ValueError("sort_tokens: num_experts must be positive and capacity not negative")
     num_experts, capacity = int(num_experts), int(capacity)
-    check_device("sort_tokens", x, expert_ids)
+    index = device_index("sort_tokens", x, expert_ids)
     if not wants_grad(x):
-        return _sort(x, expert_ids, num_experts, capacity, out)
+        return _sort(index, x, expert_ids, num_experts, capacity, out)
     if out is not None:
         raise ValueError("sort_tokens: out cannot be given where x requires a gradient")
     _not_while_capturing("sort_tokens", "sort_tokens on detached tensors and unsort_tokens for its gradient")
@@ -205,31 +201,39 @@ def _check_unsort(name, y, inverse_perm, weights, shared):
     H = _check_rows(name, y)
     T, K = _check_ids(name, inverse_perm)
     if weights is not None:
-        if weights.dtype != torch.float32:
+        if weights.dtype is not torch.float32:
             raise TypeError(f"{name}: weights must be float32")
-        if weights.shape != inverse_perm.shape:
+        if weights.shape != (T, K):
             raise ValueError(f"{name}: weights must be [T, K] like inverse_perm")
     if shared is not None:
-        if shared.dtype != y.dtype:
+        if shared.dtype is not y.dtype:
             raise TypeError(f"{name}: the [T, H] tensor must have the type of the rows")
         if shared.shape != (T, H) and (shared.dim() < 1 or shared.shape[-1] != H or shared.numel() != T * H):
             raise ValueError(f"{name}: expected a tensor of T = {T} rows of {H}")
     return T, K, H
 
 
-def _unsort(y, inverse_perm, weights, shared, out):
+def _unsort(index, y, inverse_perm, weights, shared, out):
     H = y.shape[-1]
     T, K = inverse_perm.shape
-    dev = y.device
-    y2 = _aligned(y if y.dim() == 2 else y.reshape(-1, H))
-    inv = inverse_perm.contiguous()
-    w = None if weights is None else weights.contiguous()
-    sh = None if shared is None else _aligned(shared if shared.dim() == 2 else shared.reshape(T, H))
-    result = torch.empty((T, H), dtype=y.dtype, device=dev) if out is None else out
-    if out is not None:
-        check_out("unsort_tokens", out, (T, H), y.dtype, dev, spans(y2, inv, w, sh), 16)
-    call(dev, _cabi.lib().moe_rd_unsort_tokens, T, H, K, ROW_DTYPE[y.dtype], _ptr(y2), y2.shape[0], _ptr(inv), _ptr(w),
-         _ptr(sh), _ptr(result))
+    y, y_at = dense(y if y.dim() == 2 else y.reshape(-1, H))
+    inv, inv_at = dense(inverse_perm)
+    w, w_at = (None, None) if weights is None else dense(weights)
+    sh, sh_at = (None, None) if shared is None else dense(shared if shared.dim() == 2 else shared.reshape(T, H))
+    R = y.shape[0]
+    dtype = y.dtype
+    if out is None:
+        result = torch.empty((T, H), dtype=dtype, device=y.device)
+        at = result.data_ptr()
+    else:
+        result = out
+        given = [(y_at, y.nbytes), (inv_at, 4 * T * K)]
+        if w is not None:
+            given.append((w_at, 4 * T * K))
+        if sh is not None:
+            given.append((sh_at, sh.nbytes))
+        at = check_out("unsort_tokens", out, (T, H), dtype, index, given, 16)
+    call(index, _cabi.lib().moe_rd_unsort_tokens, T, H, K, ROW_DTYPE[dtype], y_at, R, inv_at, w_at, sh_at, at)
     if out is not None:
         written(out)
     return result
@@ -238,7 +242,7 @@ def _unsort(y, inverse_perm, weights, shared, out):
 class _UnsortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, inverse_perm, weights, shared, offsets):
-        out = _unsort(y, inverse_perm, weights, shared, None)
+        out = _unsort(y.get_device(), y, inverse_perm, weights, shared, None)
         need_w = weights is not None and ctx.needs_input_grad[2]
         ctx.save_for_backward(y if need_w else None, inverse_perm, weights, offsets)
         ctx.y_shape = y.shape
@@ -253,7 +257,7 @@ class _UnsortTokens(torch.autograd.Function):
         need_y, need_w = ctx.needs_input_grad[0], weights is not None and ctx.needs_input_grad[2]
         grad_y = grad_w = grad_shared = None
         if need_y or need_w:
-            grad_y, grad_w = _unsort_backward(grad_out, y, ctx.y_shape, inverse_perm, weights, offsets, need_y, need_w, None)
+            grad_y, grad_w = _unsort_backward(grad_out.get_device(), grad_out, y, ctx.y_shape, inverse_perm, weights, offsets, need_y, need_w, None)
         if ctx.needs_input_grad[3]:
             grad_shared = grad_out.reshape(ctx.shared_shape)
         return grad_y, None, grad_w, grad_shared, None
@@ -274,47 +278,52 @@ def unsort_tokens(y: torch.Tensor, inverse_perm: torch.Tensor, weights: Optional
     required).
     """
     T, K, H = _check_unsort("unsort_tokens", y, inverse_perm, weights, shared)
-    check_device("unsort_tokens", y, inverse_perm, weights, shared, offsets)
-    _check_offsets("unsort_tokens", offsets)
+    index = device_index("unsort_tokens", y, inverse_perm, weights, shared, offsets)
+    if offsets is not None:
+        check_offsets("unsort_tokens", offsets)
     if not wants_grad(y, weights, shared):
-        return _unsort(y, inverse_perm, weights, shared, out)
+        return _unsort(index, y, inverse_perm, weights, shared, out)
     if out is not None:
         raise ValueError("unsort_tokens: out cannot be given where a gradient is required")
     _not_while_capturing("unsort_tokens", "unsort_tokens on detached tensors and unsort_tokens_backward")
     return _UnsortTokens.apply(y, inverse_perm, weights, shared, offsets)
 
 
-def _check_offsets(name, offsets):
-    if offsets is not None and (offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() < 1 or not offsets.is_contiguous()):
+def check_offsets(name, offsets):
+    if offsets.dtype is not torch.int32 or offsets.dim() != 1 or offsets.numel() < 1 or not offsets.is_contiguous():
         raise TypeError(f"{name}: offsets must be a contiguous [E+1] int32 tensor")
 
 
-def _unsort_backward(grad_out, y, y_shape, inverse_perm, weights, offsets, need_y, need_w, out):
+def _unsort_backward(index, grad_out, y, y_shape, inverse_perm, weights, offsets, need_y, need_w, out):
     T, K = inverse_perm.shape
     H = y_shape[-1]
     R = 1
     for n in y_shape[:-1]:
         R *= n
-    dev = grad_out.device
-    g = _aligned(grad_out if grad_out.dim() == 2 else grad_out.reshape(T, H))
-    y2 = None if not need_w else _aligned(y if y.dim() == 2 else y.reshape(R, H))
-    inv = inverse_perm.contiguous()
-    w = None if weights is None else weights.contiguous()
+    g, g_at = dense(grad_out if grad_out.dim() == 2 else grad_out.reshape(T, H))
+    y, y_at = dense(y if y.dim() == 2 else y.reshape(R, H)) if need_w else (None, None)
+    inv, inv_at = dense(inverse_perm)
+    w, w_at = (None, None) if weights is None else dense(weights)
+    dtype = g.dtype
+    end_at = None if offsets is None else offsets.data_ptr() + 4 * (offsets.numel() - 1)
+    rows_at = weights_at = None
     if out is None:
-        result = UnsortGradients(torch.empty(y_shape, dtype=g.dtype, device=dev) if need_y else None,
-                                 torch.empty((T, K), dtype=torch.float32, device=dev) if need_w else None)
+        result = UnsortGradients(torch.empty(y_shape, dtype=dtype, device=g.device) if need_y else None,
+                                 torch.empty((T, K), dtype=torch.float32, device=g.device) if need_w else None)
+        rows_at = result.rows.data_ptr() if need_y else None
+        weights_at = result.weights.data_ptr() if need_w else None
     else:
         result = out
         if (out.rows is not None) != need_y or (out.weights is not None) != need_w:
             raise ValueError("unsort_tokens_backward: out must hold the gradients that are asked for")
-        given = spans(g, y2, inv, w, offsets)
+        given = [(t_at, t.nbytes) for t, t_at in ((g, g_at), (y, y_at), (inv, inv_at), (w, w_at)) if t is not None]
+        if end_at is not None:
+            given.append((end_at, 4))
         if need_y:
-            check_out("unsort_tokens_backward", out.rows, y_shape, g.dtype, dev, given, 16)
+            rows_at = check_out("unsort_tokens_backward", out.rows, y_shape, dtype, index, given, 16)
         if need_w:
-            check_out("unsort_tokens_backward", out.weights, (T, K), torch.float32, dev, given)
-    n_rows = None if offsets is None else offsets.data_ptr() + 4 * (offsets.numel() - 1)
-    call(dev, _cabi.lib().moe_rd_unsort_tokens_backward, T, H, K, ROW_DTYPE[g.dtype], _ptr(g), _ptr(y2), R, _ptr(inv), _ptr(w),
-         n_rows, _ptr(result.rows), _ptr(result.weights))
+            weights_at = check_out("unsort_tokens_backward", out.weights, (T, K), torch.float32, index, given)
+    call(index, _cabi.lib().moe_rd_unsort_tokens_backward, T, H, K, ROW_DTYPE[dtype], g_at, y_at, R, inv_at, w_at, end_at, rows_at, weights_at)
     if out is not None:
         written(*out)
     return result
@@ -330,56 +339,76 @@ def unsort_tokens_backward(grad_out: torch.Tensor, y: torch.Tensor, inverse_perm
     gradient.  ``out`` takes the result of an earlier call of the same sizes."""
     need_weights = weights is not None if need_weights is None else need_weights
     _check_unsort("unsort_tokens_backward", y, inverse_perm, weights, grad_out)
-    _check_offsets("unsort_tokens_backward", offsets)
+    if offsets is not None:
+        check_offsets("unsort_tokens_backward", offsets)
     if not (need_rows or need_weights):
         raise ValueError("unsort_tokens_backward: no gradient is asked for")
-    check_device("unsort_tokens_backward", grad_out, y, inverse_perm, weights, offsets)
-    return _unsort_backward(grad_out, y, y.shape, inverse_perm, weights, offsets, need_rows, need_weights, out)
+    index = device_index("unsort_tokens_backward", grad_out, y, inverse_perm, weights, offsets)
+    return _unsort_backward(index, grad_out, y, y.shape, inverse_perm, weights, offsets, need_rows, need_weights, out)
 
 
 # --- routing weights -------------------------------------------------------------------------------------------------
 def _check_weights(name, logits, expert_ids, bias, bias_mode, score_fn):
-    if logits.dtype != torch.float32:
+    if logits.dtype is not torch.float32:
         raise TypeError(f"{name}: logits must be float32")
     T, K = _check_ids(name, expert_ids)
-    if logits.dim() != 2 or logits.shape[0] != T or logits.shape[1] < 1:
+    shape = logits.shape
+    if len(shape) != 2 or shape[0] != T or shape[1] < 1:
         raise ValueError(f"{name}: logits must be [T, E] for the T = {T} tokens of expert_ids")
     if score_fn not in SCORE_FN:
         raise ValueError(f"{name}: score_fn must be one of {tuple(SCORE_FN)}")
     if bias_mode not in BIAS_MODES:
         raise ValueError(f"{name}: bias_mode must be one of {BIAS_MODES}")
-    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != logits.shape[1]):
-        raise ValueError(f"{name}: bias must be a float32 tensor of E elements")
-    if bias is not None and wants_grad(bias):
-        raise ValueError(f"{name}: bias is a constant here; add a learned bias to the logits")
+    if bias is not None:
+        if bias.dtype is not torch.float32 or bias.numel() != shape[1]:
+            raise ValueError(f"{name}: bias must be a float32 tensor of E elements")
+        if wants_grad(bias):
+            raise ValueError(f"{name}: bias is a constant here; add a learned bias to the logits")
 
 
-def _weights_call(entry, logits, expert_ids, bias, bias_mode, score_fn, renorm, routed_scale, norm_min, *rest):
+def _weights_call(name, entry, index, logits, expert_ids, bias, config, grad, shape, out):
+    """One of the two kernels; ``shape`` is that of its result."""
+    bias_mode, score_fn, renorm, routed_scale, norm_min = config
     T, E = logits.shape
-    lg = logits.contiguous()
-    ids = expert_ids.contiguous()
-    b = None if bias is None else bias.contiguous()
-    call(logits.device, entry, T, E, ids.shape[1], SCORE_FN[score_fn], int(bool(renorm)), float(routed_scale), float(norm_min), _ptr(lg),
-         _ptr(ids), _ptr(b) if bias_mode == "logit" else None, _ptr(b) if bias_mode == "select_and_weight" else None, *map(_ptr, rest))
+    logits, logits_at = dense(logits)
+    ids, ids_at = dense(expert_ids)
+    given = [(logits_at, 4 * T * E), (ids_at, ids.nbytes)]
+    bias_at, inputs = None, ()
+    if bias is not None:
+        bias, bias_at = dense(bias)
+        given.append((bias_at, 4 * E))
+    if grad is not None:
+        grad, grad_at = dense(grad)
+        given.append((grad_at, grad.nbytes))
+        inputs = (grad_at,)
+    if out is None:
+        result = torch.empty(shape, dtype=torch.float32, device=logits.device)
+        at = result.data_ptr()
+    else:
+        result = out
+        at = check_out(name, out, shape, torch.float32, index, given)
+    call(index, entry, T, E, ids.shape[1], SCORE_FN[score_fn], 1 if renorm else 0, routed_scale, norm_min, logits_at, ids_at,
+         bias_at if bias_mode == "logit" else None, bias_at if bias_mode == "select_and_weight" else None, *inputs, at)
+    if out is not None:
+        written(out)
+    return result
 
 
 class _RoutingWeights(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, expert_ids, bias, config):
-        out = torch.empty(expert_ids.shape, dtype=torch.float32, device=logits.device)
-        _weights_call(_cabi.lib().moe_rd_routing_weights, logits, expert_ids, bias, *config, out)
         ctx.save_for_backward(logits, expert_ids, bias)
         ctx.config = config
-        return out
+        return _weights_call("routing_weights", _cabi.lib().moe_rd_routing_weights, logits.get_device(), logits, expert_ids, bias, config, None,
+                             expert_ids.shape, None)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         _not_while_capturing("routing_weights", "routing_weights on detached logits and routing_weights_backward")
         logits, expert_ids, bias = ctx.saved_tensors
-        out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
-        _weights_call(_cabi.lib().moe_rd_routing_weights_backward, logits, expert_ids, bias, *ctx.config, grad.contiguous(), out)
-        return out, None, None, None
+        return _weights_call("routing_weights", _cabi.lib().moe_rd_routing_weights_backward, logits.get_device(), logits, expert_ids, bias,
+                             ctx.config, grad, logits.shape, None), None, None, None
 
 
 def routing_weights(logits: torch.Tensor, expert_ids: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -393,22 +422,15 @@ def routing_weights(logits: torch.Tensor, expert_ids: torch.Tensor, bias: Option
     ``logits = x @ gate_weight`` it carries the gradient of the weights to the router.
     """
     _check_weights("routing_weights", logits, expert_ids, bias, bias_mode, score_fn)
-    dev = check_device("routing_weights", logits, expert_ids, bias)
+    index = device_index("routing_weights", logits, expert_ids, bias)
     config = (bias_mode, score_fn, renorm, routed_scale, norm_min)
     if wants_grad(logits):
         if out is not None:
             raise ValueError("routing_weights: out cannot be given where a gradient is required")
         _not_while_capturing("routing_weights", "routing_weights on detached logits and routing_weights_backward")
         return _RoutingWeights.apply(logits, expert_ids, bias, config)
-    if out is None:
-        result = torch.empty(expert_ids.shape, dtype=torch.float32, device=dev)
-    else:
-        result = out
-        check_out("routing_weights", out, expert_ids.shape, torch.float32, dev, spans(logits, expert_ids, bias))
-    _weights_call(_cabi.lib().moe_rd_routing_weights, logits, expert_ids, bias, *config, result)
-    if out is not None:
-        written(out)
-    return result
+    return _weights_call("routing_weights", _cabi.lib().moe_rd_routing_weights, index, logits, expert_ids, bias, config, None,
+                         expert_ids.shape, out)
 
 
 def routing_weights_backward(grad_weights: torch.Tensor, logits: torch.Tensor, expert_ids: torch.Tensor,
@@ -419,17 +441,8 @@ def routing_weights_backward(grad_weights: torch.Tensor, logits: torch.Tensor, e
     the sum of the chosen scores is below ``norm_min`` it has no part in the gradient; a token without any valid id gets
     zeros."""
     _check_weights("routing_weights_backward", logits, expert_ids, bias, bias_mode, score_fn)
-    if grad_weights.dtype != torch.float32 or grad_weights.shape != expert_ids.shape:
+    if grad_weights.dtype is not torch.float32 or grad_weights.shape != expert_ids.shape:
         raise ValueError("routing_weights_backward: grad_weights must be a float32 tensor like expert_ids")
-    dev = check_device("routing_weights_backward", logits, grad_weights, expert_ids, bias)
-    grad = grad_weights.contiguous()
-    if out is None:
-        result = torch.empty(logits.shape, dtype=torch.float32, device=dev)
-    else:
-        result = out
-        check_out("routing_weights_backward", out, logits.shape, torch.float32, dev, spans(logits, expert_ids, bias, grad))
-    _weights_call(_cabi.lib().moe_rd_routing_weights_backward, logits, expert_ids, bias, bias_mode, score_fn, renorm, routed_scale,
-                  norm_min, grad, result)
-    if out is not None:
-        written(out)
-    return result
+    index = device_index("routing_weights_backward", logits, grad_weights, expert_ids, bias)
+    return _weights_call("routing_weights_backward", _cabi.lib().moe_rd_routing_weights_backward, index, logits, expert_ids, bias,
+                         (bias_mode, score_fn, renorm, routed_scale, norm_min), grad_weights, logits.shape, out)
