@@ -151,7 +151,9 @@ __device__ __forceinline__ void unpack8(const uint4& v, float f[8]) {
 }
 
 // exp(x) from IEEE operations only (no MUFU): n = rint(x*log2 e), two-step
-// Cody-Waite reduction, degree-6 polynomial, scale through the exponent field.
+// Cody-Waite reduction, degree-6 polynomial (the single-precision coefficients of
+// S. L. Moshier, Methods and Programs for Mathematical Functions, 1989), scale
+// through the exponent field.
 __device__ __forceinline__ float exp_ieee(float x) {
   if (x < -87.0f) return 0.0f;
   if (x > 88.0f) return __int_as_float(0x7f800000);
