@@ -7,9 +7,13 @@
 // * batch: sort_count_kernel counts the pairs per (tile of 64 tokens, expert) and per (group of 32 tiles, expert);
 //   positions_kernel and scatter_kernel of the routing pipeline (scatter.cu) derive the places from those counts and
 //   copy the rows, each token row read once and stored K times.
-// * up to kOncePairs pairs and kOnceBytes of rows: one kernel.  Every block counts ALL pairs by itself (how many of every expert there are, and
-//   how many before its own tokens), ranks its own pairs and copies their rows: the counting is done hundreds of times
-//   over, but from L2 and by blocks that would otherwise wait, and one launch does the work of three.  No workspace.
+// * up to kOncePairs pairs and kOnceBytes of rows: one kernel.  Every block counts ALL pairs by itself (how many of every
+//   expert there are, and how many before its own tokens), ranks its own pairs and copies their rows: the counting is
+//   done hundreds of times over, but from L2 and by blocks that would otherwise wait, and one launch does the work of
+//   three.  No workspace.
+// The counts are shared-memory atomics (their order does not matter); with __match_any_sync and one atomic per distinct
+// expert 16384 pairs of 256 experts took 85 us instead of 13.
+// Batch: 8192 tokens x 7168 bf16, K = 8: 172 us, 6.1 TB/s, of which about 8 us are the counts and places.
 #include "row_types.cuh"
 
 namespace moe_rd {

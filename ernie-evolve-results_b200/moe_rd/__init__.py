@@ -9,6 +9,12 @@ registered as the torch custom op ``torch.ops.moe_rd.route_dispatch`` (CUDA
 only) on top of the C ABI in ``include/moe_rd.h``.  There is no CPU fallback
 and no alternative backend: without ``libmoe_rd.so`` or without a CUDA device
 every call raises.
+
+Around that call: ``combine`` and its relatives (the way back), the parts of the
+path for training and for routings that come from elsewhere (``sort_tokens``,
+``unsort_tokens``, ``routing_weights``, each with its gradient; see
+``moe_rd.sorting``) and the 4-bit expert products of a decode step
+(``pack_w4``, ``expert_matvec_w4``; see ``moe_rd.experts``).
 """
 from __future__ import annotations
 
