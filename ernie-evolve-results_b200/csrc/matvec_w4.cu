@@ -216,11 +216,9 @@ struct W4Joint {
   int expert[kMaxE], lo[kMaxE], n[kMaxE], unit[kMaxE];  // experts that have rows: number, rows, units before
 };
 
-// The units that several warps have: a thread per sum, 256 a unit, added in the order of the warps.  Called once with
-// rows = 0, which writes nothing, while the first tiles are on their way: the instructions would otherwise have to be
-// fetched through a memory system that is busy with weights, 2 us at the end of every call.
+// The units that several warps have: a thread per sum, 256 a unit, added in the order of the warps.
 template <int DT>
-__device__ __noinline__ void w4_join(const W4Args& a, const W4Joint& s, int rows) {
+__device__ __forceinline__ void w4_join(const W4Args& a, const W4Joint& s) {
   const int tid = threadIdx.x, lane = tid & 31;
   const int what = lane < kW4Warps ? s.what[lane] : 0;
   const unsigned continues = __ballot_sync(kFull, what & kContinues), ends = __ballot_sync(kFull, what & kEnds);
@@ -235,7 +233,7 @@ __device__ __noinline__ void w4_join(const W4Args& a, const W4Joint& s, int rows
 #pragma unroll
     for (int v = 1; v < kW4Warps; ++v)
       if (v > w && v <= last && ((continues >> v) & 1u)) sum = __fadd_rn(sum, s.sum[v][el]);
-    if (r < min(rows, s.n[p.i]) && col < a.N) reinterpret_cast<uint16_t*>(a.out)[(size_t)(s.lo[p.i] + r) * a.N + col] = W4Type<DT>::round(sum);
+    if (r < s.n[p.i] && col < a.N) reinterpret_cast<uint16_t*>(a.out)[(size_t)(s.lo[p.i] + r) * a.N + col] = W4Type<DT>::round(sum);
   }
 }
 
@@ -298,10 +296,6 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
   if (broken) {
     units = 0;
     first_row = last_row = 0;
-  }
-  if (tid < kW4Warps) {  // for the call of w4_join that writes nothing
-    s.what[tid] = tid < kW4Threads / 256 ? kBegins : kContinues | kEnds;
-    s.place[tid] = W4Place{0, 0, 0, 0};
   }
   __syncthreads();
 
@@ -370,8 +364,6 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
   if (count > 0) aim();
 #pragma unroll 1
   for (int d = 0; d < kDepth; ++d) fetch(d * St::kBytes);
-  w4_join<DT>(a, s, 0);
-  __syncthreads();
 
   float acc[2][4];
   const unsigned char* xp = nullptr;
@@ -460,7 +452,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
     s.place[warp] = here;
   }
   __syncthreads();
-  w4_join<DT>(a, s, INT_MAX);
+  w4_join<DT>(a, s);
 
   // rows of no expert
   const int64_t before = (int64_t)first_row * a.N, idle = before + (a.rows - last_row) * a.N;
