@@ -30,6 +30,7 @@ class UnsortGradients(NamedTuple):
     weights: Optional[torch.Tensor]  # [T, K] fp32 gradient of the weights
 
 
+_increment_version = torch.autograd.graph.increment_version
 _VECTOR = {torch.bfloat16: 8, torch.float16: 8, torch.float32: 4}  # elements in 16 bytes
 
 
@@ -74,9 +75,8 @@ def check_out(name: str, out: torch.Tensor, shape: Tuple[int, ...], dtype: torch
     lo = out.data_ptr()
     if lo % align:
         raise ValueError(f"{name}: out must be {align}-byte aligned")
-    hi = lo + out.nbytes
     for at, nbytes in inputs:
-        if lo < at + nbytes and at < hi:
+        if lo < at + nbytes and at < lo + out.nbytes:
             raise ValueError(f"{name}: out must not share memory with an input")
     return lo
 
@@ -84,7 +84,7 @@ def check_out(name: str, out: torch.Tensor, shape: Tuple[int, ...], dtype: torch
 def written(*out: Optional[torch.Tensor]) -> None:
     """Tell autograd that these buffers of the caller have been overwritten: a graph that saved one of them then raises in
     its backward pass instead of computing with the new contents."""
-    torch.autograd.graph.increment_version([t for t in out if t is not None])
+    _increment_version([t for t in out if t is not None])
 
 
 def wants_grad(*tensors: Optional[torch.Tensor]) -> bool:
@@ -121,10 +121,7 @@ def _check_rows(name: str, rows: torch.Tensor) -> int:
 
 
 # --- sort ------------------------------------------------------------------------------------------------------------
-def _sort(index, x, expert_ids, num_experts, capacity, out):
-    H = x.shape[-1]
-    T, K = expert_ids.shape
-    E = num_experts
+def _sort(index, T, K, H, x, expert_ids, E, capacity, out):
     x, x_at = dense(x if x.dim() == 2 else x.reshape(T, H))
     ids, ids_at = dense(expert_ids)
     R = min(T * K, E * capacity) if capacity else T * K
@@ -146,14 +143,14 @@ def _sort(index, x, expert_ids, num_experts, capacity, out):
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
     call(index, _cabi.lib().moe_rd_sort_tokens, T, H, E, K, code, capacity, R, x_at, ids_at, *at, ws.data_ptr() if ws_bytes else None, ws_bytes)
     if out is not None:
-        written(*out)
+        _increment_version(out)
     return result
 
 
 class _SortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, expert_ids, num_experts, capacity):
-        out = _sort(x.get_device(), x, expert_ids, num_experts, capacity, None)
+        out = _sort(x.get_device(), *expert_ids.shape, x.shape[-1], x, expert_ids, num_experts, capacity, None)
         ctx.save_for_backward(out.inverse_perm)
         ctx.shape = x.shape
         ctx.mark_non_differentiable(*out[1:])
@@ -164,7 +161,8 @@ class _SortTokens(torch.autograd.Function):
     def backward(ctx, grad_rows, *_):
         _not_while_capturing("sort_tokens", "sort_tokens on detached tensors and unsort_tokens for its gradient")
         (inverse_perm,) = ctx.saved_tensors
-        return _unsort(grad_rows.get_device(), grad_rows, inverse_perm, None, None, None).reshape(ctx.shape), None, None, None
+        grad = _unsort(grad_rows.get_device(), *inverse_perm.shape, ctx.shape[-1], grad_rows, inverse_perm, None, None, None)
+        return grad.reshape(ctx.shape), None, None, None
 
 
 def sort_tokens(x: torch.Tensor, expert_ids: torch.Tensor, num_experts: int, *, capacity: int = 0,
@@ -189,7 +187,7 @@ def sort_tokens(x: torch.Tensor, expert_ids: torch.Tensor, num_experts: int, *, 
     num_experts, capacity = int(num_experts), int(capacity)
     index = device_index("sort_tokens", x, expert_ids)
     if not wants_grad(x):
-        return _sort(index, x, expert_ids, num_experts, capacity, out)
+        return _sort(index, T, K, H, x, expert_ids, num_experts, capacity, out)
     if out is not None:
         raise ValueError("sort_tokens: out cannot be given where x requires a gradient")
     _not_while_capturing("sort_tokens", "sort_tokens on detached tensors and unsort_tokens for its gradient")
@@ -213,9 +211,7 @@ def _check_unsort(name, y, inverse_perm, weights, shared):
     return T, K, H
 
 
-def _unsort(index, y, inverse_perm, weights, shared, out):
-    H = y.shape[-1]
-    T, K = inverse_perm.shape
+def _unsort(index, T, K, H, y, inverse_perm, weights, shared, out):
     y, y_at = dense(y if y.dim() == 2 else y.reshape(-1, H))
     inv, inv_at = dense(inverse_perm)
     w, w_at = (None, None) if weights is None else dense(weights)
@@ -235,14 +231,14 @@ def _unsort(index, y, inverse_perm, weights, shared, out):
         at = check_out("unsort_tokens", out, (T, H), dtype, index, given, 16)
     call(index, _cabi.lib().moe_rd_unsort_tokens, T, H, K, ROW_DTYPE[dtype], y_at, R, inv_at, w_at, sh_at, at)
     if out is not None:
-        written(out)
+        _increment_version(out)
     return result
 
 
 class _UnsortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, inverse_perm, weights, shared, offsets):
-        out = _unsort(y.get_device(), y, inverse_perm, weights, shared, None)
+        out = _unsort(y.get_device(), *inverse_perm.shape, y.shape[-1], y, inverse_perm, weights, shared, None)
         need_w = weights is not None and ctx.needs_input_grad[2]
         ctx.save_for_backward(y if need_w else None, inverse_perm, weights, offsets)
         ctx.y_shape = y.shape
@@ -282,7 +278,7 @@ def unsort_tokens(y: torch.Tensor, inverse_perm: torch.Tensor, weights: Optional
     if offsets is not None:
         check_offsets("unsort_tokens", offsets)
     if not wants_grad(y, weights, shared):
-        return _unsort(index, y, inverse_perm, weights, shared, out)
+        return _unsort(index, T, K, H, y, inverse_perm, weights, shared, out)
     if out is not None:
         raise ValueError("unsort_tokens: out cannot be given where a gradient is required")
     _not_while_capturing("unsort_tokens", "unsort_tokens on detached tensors and unsort_tokens_backward")
@@ -390,7 +386,7 @@ def _weights_call(name, entry, index, logits, expert_ids, bias, config, grad, sh
     call(index, entry, T, E, ids.shape[1], SCORE_FN[score_fn], 1 if renorm else 0, routed_scale, norm_min, logits_at, ids_at,
          bias_at if bias_mode == "logit" else None, bias_at if bias_mode == "select_and_weight" else None, *inputs, at)
     if out is not None:
-        written(out)
+        _increment_version(out)
     return result
 
 

@@ -195,3 +195,24 @@ def test_graph_and_other_stream():
     # rows that are a view: strided, and starting off a 16-byte boundary
     wide = torch.randn(6, 520).to(torch.bfloat16).cuda()
     assert torch.equal(moe_rd.expert_matvec_w4(wide[:, 3:515], packed, off), moe_rd.expert_matvec_w4(wide[:, 3:515].clone(), packed, off))
+
+
+def test_weights_past_32_bits():
+    """More than 2^32 bytes of weights: the last expert's last outputs."""
+    E, N, K, group = 130, 8192, 8192, 128
+    q = torch.randint(0, 256, (E, N, K // 2), device="cuda", dtype=torch.uint8)
+    s = (torch.rand(E, N, K // group, device="cuda") / 64).to(torch.bfloat16)
+    packed = moe_rd.pack_w4(q, s)
+    assert packed.packed.numel() > 2 ** 32
+    off = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+    off[1:] = 1
+    off[-1] = 3
+    x = torch.randn(3, K, device="cuda").to(torch.bfloat16)
+    got = moe_rd.expert_matvec_w4(x, packed, off)
+    for rows, e in (([0], 0), ([1, 2], E - 1)):
+        w = torch.stack([q[e] & 15, q[e] >> 4], -1).reshape(N, K // group, group).double() - 8.0
+        w = (w * s[e].double()[..., None]).reshape(N, K)
+        want = x[rows].double() @ w.t()
+        err = (got[rows].double() - want).abs()
+        low = (8 * 17 + 2 * (K / 32) + 16) * 2.0 ** -24 * (x[rows].double().abs() @ w.abs().t())
+        assert (err <= low + 2.0 ** -8 * (want.abs() + low)).all()

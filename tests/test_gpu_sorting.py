@@ -415,3 +415,73 @@ def test_out_is_checked():
         moe_rd.sort_tokens(x, ids.cpu(), 8)
     with pytest.raises(moe_rd.MoeRdError):
         moe_rd.sort_tokens(x, ids, 257)
+
+
+def test_rows_past_32_bits():
+    """More than 2^31 elements, more than 2^32 bytes of rows: the far end of every buffer is reached."""
+    T, K, E, H = 38000, 8, 256, 7168
+    assert T * K * H > 2 ** 31
+    x = torch.randn(T, H, device="cuda").to(torch.bfloat16)
+    ids = torch.randint(0, E, (T, K), device="cuda", dtype=torch.int32)
+    ids[::5] = -1
+    s = moe_rd.sort_tokens(x, ids, E)
+    live = int(s.offsets[-1])
+    assert (s.inverse_perm[::5] == -1).all() and int((s.inverse_perm >= 0).sum()) == live
+    probe = torch.cat([torch.arange(0, 300), torch.arange(live - 300, live)]).cuda()
+    assert torch.equal(s.rows[probe], x[s.row_token[probe].long()])
+    assert (s.rows[live:][-200:] == 0).all() and (s.row_token[live:] == -1).all()
+    w = torch.rand(T, K, device="cuda")
+    back = moe_rd.unsort_tokens(s.rows, s.inverse_perm, w)
+    some = torch.tensor([0, 1, 5, T // 2, T - 2, T - 1]).cuda()
+    want = x[some].double() * (w[some].double().sum(1) * (ids[some, 0] >= 0))[:, None]
+    low = K * 2.0 ** -24 * (1 + K * 2.0 ** -24) * want.abs()    # K additions of one sign in 32 bits, then one rounding
+    assert ((back[some].double() - want).abs() <= low + 2.0 ** -8 * (want.abs() + low)).all()
+    g = moe_rd.unsort_tokens_backward(x, s.rows, s.inverse_perm, w, offsets=s.offsets)
+    at = s.row_token[probe].long()
+    k = (s.inverse_perm[at] == probe[:, None].int()).int().argmax(1)
+    want = x[at].double() * w[at, k].double()[:, None]
+    assert ((g.rows[probe].double() - want).abs() <= (2.0 ** -8 + 2.0 ** -23) * want.abs() + 1e-38).all()
+    assert (g.rows[live:][-200:] == 0).all()
+    norm = (x[at].double() ** 2).sum(1)
+    assert ((g.weights[at, k].double() - norm).abs() <= (H / 32 + 21) * 2.0 ** -24 * norm).all()
+
+
+def test_batches_of_any_shape_through_autograd():
+    """x and the shared branch as [batch, length, H], strided; gradients arrive in their shapes."""
+    base = torch.randn(3, 10, 2, 64, device="cuda", requires_grad=True)
+    x = base[:, :, 1]
+    ids = ids_of(30, 2, 4, "padded").cuda()
+    s = moe_rd.sort_tokens(x, ids, 4)
+    out = moe_rd.unsort_tokens(s.rows * 2, s.inverse_perm, None, x, offsets=s.offsets)
+    out.sum().backward()
+    n = (ids >= 0).sum(1).float().view(3, 10, 1)
+    want = torch.zeros_like(base)
+    want[:, :, 1] = (1 + 2 * n).expand(3, 10, 64)
+    assert torch.equal(base.grad, want)
+
+
+def test_two_threads_on_two_streams():
+    import threading
+    T, K, E, H = 3000, 4, 64, 256
+    data = [(torch.randn(T, H, device="cuda"), ids_of(T, K, E, "padded", i).cuda()) for i in range(2)]
+    want = [moe_rd.sort_tokens(x, ids, E) for x, ids in data]
+    want_back = [moe_rd.unsort_tokens(w.rows, w.inverse_perm) for w in want]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                s = moe_rd.sort_tokens(*data[i], E)
+                b = moe_rd.unsort_tokens(s.rows, s.inverse_perm)
+                few = moe_rd.sort_tokens(data[i][0][:100], data[i][1][:100], E)
+            torch.cuda.current_stream().synchronize()
+            if not (all(torch.equal(p, q) for p, q in zip(s, want[i])) and torch.equal(b, want_back[i]) and few.rows.shape == (400, H)):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
