@@ -20,7 +20,7 @@
 // The copies alone run at 6.7 TB/s (64 experts x 4096 x 7168: 145 us), the kernel at 5.5 (175 us): what bounds it is the
 // integer pipe, 7 instructions for 8 bf16 weights (5 for fp16, 6 % faster).
 //
-// A unit of work is 32 outputs of one expert for up to eight of its rows; its tiles lie one behind the other in memory,
+// A unit of work is 32 outputs of one expert for up to eight (or 16, see launch_w4_rows) of its rows; its tiles lie one behind the other in memory,
 // and so do the units of an expert.  Only experts that have rows get units: every block lists them from the offsets.  A
 // block gets a run of whole units, and its warps equal shares of the run's tiles, cut anywhere: a warp streams one
 // contiguous stretch of weights, kDepth tiles ahead of its products (cp.async into its own part of shared memory; it
@@ -141,35 +141,44 @@ struct W4Type<MOE_RD_T_FP16> {
   }
 };
 
-// acc += the product of one tile: w[2s + h] are the words of outputs 16s + 8h + g, x[q] the lane's inputs of block q,
-// scale(k, i) and zero(k, i) those of group k of the tile and output 8i + g.
-template <int DT, int SPAN, typename Scale, typename Zero>
-__device__ __forceinline__ void w4_tile(const W4Type<DT>& ty, const uint4 (&w)[4], const uint4 (&x)[4], Scale scale, Zero zero,
-                                        float (&acc)[2][4]) {
+// acc += the product of one tile: w[2s + h] are the words of outputs 16s + 8h + g, x(q, v) the lane's inputs of block q for
+// rows 8v.., scale(k, i) and zero(k, i) those of group k of the tile and output 8i + g.
+template <int DT, int SPAN, int NT, typename X, typename Scale, typename Zero>
+__device__ __forceinline__ void w4_tile(const W4Type<DT>& ty, const uint4 (&w)[4], X x, Scale scale, Zero zero,
+                                        float (&acc)[2][NT][4]) {
   using Ty = W4Type<DT>;
   const uint32_t word[4][4] = {{w[0].x, w[0].y, w[0].z, w[0].w}, {w[1].x, w[1].y, w[1].z, w[1].w},
                                {w[2].x, w[2].y, w[2].z, w[2].w}, {w[3].x, w[3].y, w[3].z, w[3].w}};
 #pragma unroll
   for (int k = 0; k < 4 / SPAN; ++k) {
-    float part[2][4];
+    float part[2][NT][4];
 #pragma unroll
     for (int q = k * SPAN; q < (k + 1) * SPAN; ++q) {
+      uint4 xq[NT];
+#pragma unroll
+      for (int v = 0; v < NT; ++v) xq[v] = x(q, v);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         uint32_t a[4], b[4];
         ty.unpack(word[2 * s][q], zero(k, 2 * s), a);
         ty.unpack(word[2 * s + 1][q], zero(k, 2 * s + 1), b);
-        if (q == k * SPAN)
-          Ty::mma(part[s], a[0], b[0], a[1], b[1], x[q].x, x[q].y, 0.0f, 0.0f, 0.0f, 0.0f);
-        else
-          Ty::mma(part[s], a[0], b[0], a[1], b[1], x[q].x, x[q].y, part[s][0], part[s][1], part[s][2], part[s][3]);
-        Ty::mma(part[s], a[2], b[2], a[3], b[3], x[q].z, x[q].w, part[s][0], part[s][1], part[s][2], part[s][3]);
+#pragma unroll
+        for (int v = 0; v < NT; ++v) {
+          float(&d)[4] = part[s][v];
+          if (q == k * SPAN)
+            Ty::mma(d, a[0], b[0], a[1], b[1], xq[v].x, xq[v].y, 0.0f, 0.0f, 0.0f, 0.0f);
+          else
+            Ty::mma(d, a[0], b[0], a[1], b[1], xq[v].x, xq[v].y, d[0], d[1], d[2], d[3]);
+          Ty::mma(d, a[2], b[2], a[3], b[3], xq[v].z, xq[v].w, d[0], d[1], d[2], d[3]);
+        }
       }
     }
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[s][i] = fmaf(scale(k, 2 * s + (i >> 1)), part[s][i], acc[s][i]);
+      for (int v = 0; v < NT; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[s][v][i] = fmaf(scale(k, 2 * s + (i >> 1)), part[s][v][i], acc[s][v][i]);
   }
 }
 
@@ -188,20 +197,25 @@ __device__ __forceinline__ uint32_t w4_group(const W4Args& a, uint32_t b) {  // 
   return a.group_magic != 0 ? __umulhi(b, a.group_magic) : b;
 }
 
+// The lane's inputs of block q of tile c, from where its inputs of the tile begin; zeros past the last input.
+__device__ __forceinline__ uint4 w4_load_x(const W4Args& a, const unsigned char* xp, int c, int q) {
+  return 128 * c + 32 * q < a.K ? __ldg(reinterpret_cast<const uint4*>(xp + 64 * q)) : make_uint4(0u, 0u, 0u, 0u);
+}
+
+// ... of all its blocks; only the last tile can have padding.
 __device__ __forceinline__ void w4_load_x(const W4Args& a, const unsigned char* xp, int c, uint4 (&x)[4]) {
   if (c < a.K >> 7) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) x[q] = __ldg(reinterpret_cast<const uint4*>(xp + 64 * q));
   } else {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      x[q] = 128 * c + 32 * q < a.K ? __ldg(reinterpret_cast<const uint4*>(xp + 64 * q)) : make_uint4(0u, 0u, 0u, 0u);
+    for (int q = 0; q < 4; ++q) x[q] = w4_load_x(a, xp, c, q);
   }
 }
 
 // Where a warp is in its share of the block's tiles.
 struct W4Place {
-  int i, nb, pass;  // expert (of the list), block of 32 outputs, pass over eight rows
+  int i, nb, pass;  // expert (of the list), block of 32 outputs, pass over 8 * NT rows
   int c;            // tile of 128 inputs
 };
 
@@ -209,26 +223,28 @@ struct W4Place {
 // part of a unit that it began itself and later warps end.
 enum { kContinues = 1, kEnds = 2, kBegins = 4 };
 
+template <int NT>
 struct W4Joint {
-  float sum[2 * kW4Warps][32 * 8];  // [warp]: the part of the first unit; [kW4Warps + warp]: of the last; [row of x][output]
+  float sum[2 * kW4Warps][256 * NT];  // [warp]: the part of the first unit; [kW4Warps + warp]: of the last; [row of x][output]
   W4Place place[kW4Warps];          // of the unit that the warp began
   int what[kW4Warps];
   int expert[kMaxE], lo[kMaxE], n[kMaxE], unit[kMaxE];  // experts that have rows: number, rows, units before
 };
 
-// The units that several warps have: a thread per sum, 256 a unit, added in the order of the warps.
-template <int DT>
-__device__ __forceinline__ void w4_join(const W4Args& a, const W4Joint& s) {
+// The units that several warps have: a thread per sum, 256 NT a unit, added in the order of the warps.
+template <int DT, int NT>
+__device__ __forceinline__ void w4_join(const W4Args& a, const W4Joint<NT>& s) {
+  constexpr int kSums = 256 * NT;
   const int tid = threadIdx.x, lane = tid & 31;
   const int what = lane < kW4Warps ? s.what[lane] : 0;
   const unsigned continues = __ballot_sync(kFull, what & kContinues), ends = __ballot_sync(kFull, what & kEnds);
   unsigned begins = __ballot_sync(kFull, what & kBegins);
   for (int k = 0; begins != 0; ++k, begins &= begins - 1) {
-    if (k % (kW4Threads / 256) != tid >> 8) continue;
+    if (k % (kW4Threads / kSums) != tid / kSums) continue;
     const int w = __ffs(begins) - 1;
     const int last = w + __ffs(ends >> (w + 1));
     const W4Place p = s.place[w];
-    const int el = tid & 255, r = p.pass * 8 + (el >> 5), col = p.nb * 32 + (el & 31);
+    const int el = tid & (kSums - 1), r = p.pass * 8 * NT + (el >> 5), col = p.nb * 32 + (el & 31);
     float sum = s.sum[kW4Warps + w][el];
 #pragma unroll
     for (int v = 1; v < kW4Warps; ++v)
@@ -237,14 +253,15 @@ __device__ __forceinline__ void w4_join(const W4Args& a, const W4Joint& s) {
   }
 }
 
-template <int DT, int SPAN, bool ZEROS>
+// NT: a unit has up to 8 NT rows; the operands of a tile are made once and multiplied NT times.
+template <int DT, int SPAN, bool ZEROS, int NT>
 __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
   using Ty = W4Type<DT>;
   using St = W4Stage<SPAN, ZEROS>;
   extern __shared__ __align__(16) unsigned char s_dynamic[];  // W4Joint, then the rings [warps][kDepth][St::kBytes]
   __shared__ int s_w[kW4Warps], s_u[kW4Warps];
-  W4Joint& s = *reinterpret_cast<W4Joint*>(s_dynamic);
-  unsigned char* s_ring = s_dynamic + sizeof(W4Joint);
+  W4Joint<NT>& s = *reinterpret_cast<W4Joint<NT>*>(s_dynamic);
+  unsigned char* s_ring = s_dynamic + sizeof(W4Joint<NT>);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, j = lane & 3;
   const Ty ty;
@@ -264,7 +281,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
     first_row = __ldg(a.offsets);
     last_row = __ldg(a.offsets + a.E);
   }
-  const int mine = n > 0 ? ((n + 7) >> 3) * a.nblocks : 0;
+  const int mine = n > 0 ? (n + 8 * NT - 1) / (8 * NT) * a.nblocks : 0;
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -315,14 +332,14 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
       if (m != kFull) break;
     }
     --here.i;
-    const int in = u - s.unit[here.i], passes = (s.n[here.i] + 7) >> 3;
+    const int in = u - s.unit[here.i], passes = (s.n[here.i] + 8 * NT - 1) / (8 * NT);
     here.nb = passes == 1 ? in : in / passes;
     here.pass = in - here.nb * passes;
   }
   // to the first tile of the next unit
   auto next_unit = [&](W4Place& p) {
     p.c = 0;
-    if (++p.pass * 8 < s.n[p.i]) return;
+    if (++p.pass * 8 * NT < s.n[p.i]) return;
     p.pass = 0;
     if (++p.nb < a.nblocks) return;
     p.nb = 0;
@@ -365,26 +382,32 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
 #pragma unroll 1
   for (int d = 0; d < kDepth; ++d) fetch(d * St::kBytes);
 
-  float acc[2][4];
-  const unsigned char* xp = nullptr;
+  float acc[2][NT][4];
+  const unsigned char* xp[NT];
   bool began = here.c == 0;  // this warp has the unit from its first tile on
   auto begin = [&]() {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int v = 0; v < NT; ++v) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[h][i] = 0.0f;
-    // columns behind the unit's last row multiply that row again; their results are dropped
-    const int row = s.lo[here.i] + min(here.pass * 8 + g, s.n[here.i] - 1);
-    xp = a.x + ((size_t)row * a.K + here.c * 128 + 8 * j) * 2;
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[h][v][i] = 0.0f;
+      // columns behind the unit's last row multiply that row again; their results are dropped
+      const int row = s.lo[here.i] + min(8 * (here.pass * NT + v) + g, s.n[here.i] - 1);
+      xp[v] = a.x + ((size_t)row * a.K + here.c * 128 + 8 * j) * 2;
+    }
   };
   auto write = [&]() {
-    const int r0 = here.pass * 8, rows = s.n[here.i] - r0, cols = a.N - here.nb * 32 - g;
+    const int r0 = here.pass * 8 * NT, rows = s.n[here.i] - r0, cols = a.N - here.nb * 32 - g;
     uint16_t* o = reinterpret_cast<uint16_t*>(a.out) + (size_t)(s.lo[here.i] + r0 + 2 * j) * a.N + here.nb * 32 + g;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (2 * j + (i & 1) < rows && 16 * h + 8 * (i >> 1) < cols) o[(size_t)(i & 1) * a.N + 16 * h + 8 * (i >> 1)] = Ty::round(acc[h][i]);
+      for (int v = 0; v < NT; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (8 * v + 2 * j + (i & 1) < rows && 16 * h + 8 * (i >> 1) < cols)
+            o[(size_t)(8 * v + (i & 1)) * a.N + 16 * h + 8 * (i >> 1)] = Ty::round(acc[h][v][i]);
   };
   int what = 0, slot = 0;  // byte offset in the ring
   for (int t = count; t > 0;) {
@@ -392,11 +415,14 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
     // the rest of this unit, or of the share
     const int stretch = min(t, a.chunks - here.c);
     t -= stretch;
-    // one tile with its inputs in `x`, while those of the next are fetched into `x_next`
     const int c_end = here.c + stretch;
+    // one tile with its inputs in `x`, while those of the next are fetched into `x_next` (NT = 1: more registers there
+    // are not, the inputs of the other rows come from L1 when their block's turn is)
     auto tile = [&](const uint4 (&x)[4], uint4 (&x_next)[4]) {
-      xp += 256;
-      if (here.c + 1 < c_end) w4_load_x(a, xp, here.c + 1, x_next);
+      if (NT == 1) {
+        xp[0] += 256;
+        if (here.c + 1 < c_end) w4_load_x(a, xp[0], here.c + 1, x_next);
+      }
       asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
       __syncwarp();  // the scales of a tile are copied by all lanes
       const unsigned char* st = ring_p + slot;
@@ -413,21 +439,26 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
       __syncwarp();
       fetch(slot);
       slot = slot + St::kBytes == kDepth * St::kBytes ? 0 : slot + St::kBytes;
-      w4_tile<DT, SPAN>(
-          ty, w, x,
+      w4_tile<DT, SPAN, NT>(
+          ty, w, [&](int q, int v) { return NT == 1 ? x[q] : w4_load_x(a, xp[v], here.c, q); },
           [&](int k, int i) {
             const uint32_t v = i < 2 ? sc[k].x : sc[k].y;
             return i & 1 ? Ty::second(v) : Ty::first(v);
           },
           [&](int k, int i) { return Ty::zero_operand((zp[k] >> (4 * i)) & 15u); }, acc);
+      if (NT > 1) {
+#pragma unroll
+        for (int v = 0; v < NT; ++v) xp[v] += 256;
+      }
       ++here.c;
     };
     uint4 x0[4], x1[4];
-    w4_load_x(a, xp, here.c, x0);
+    if (NT == 1) w4_load_x(a, xp[0], here.c, x0);
 #pragma unroll 1
     while (true) {
       tile(x0, x1);
       if (here.c == c_end) break;
+      if (NT > 1) continue;
       tile(x1, x0);
       if (here.c == c_end) break;
     }
@@ -439,7 +470,9 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) to[(2 * j + (i & 1)) * 32 + 16 * h + 8 * (i >> 1) + g] = acc[h][i];
+        for (int v = 0; v < NT; ++v)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) to[(8 * v + 2 * j + (i & 1)) * 32 + 16 * h + 8 * (i >> 1) + g] = acc[h][v][i];
       what |= began ? kBegins : ended ? kContinues | kEnds : kContinues;
     }
     if (t > 0) {
@@ -452,7 +485,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
     s.place[warp] = here;
   }
   __syncthreads();
-  w4_join<DT>(a, s);
+  w4_join<DT, NT>(a, s);
 
   // rows of no expert
   const int64_t before = (int64_t)first_row * a.N, idle = before + (a.rows - last_row) * a.N;
@@ -482,28 +515,36 @@ __global__ void __launch_bounds__(256) pack_w4_kernel(const unsigned char* __res
   }
 }
 
-template <int DT, int SPAN, bool ZEROS>
+template <int DT, int SPAN, bool ZEROS, int NT>
 cudaError_t launch_w4(const W4Args& a, cudaStream_t s) {
-  constexpr int smem = sizeof(W4Joint) + kW4Warps * kDepth * W4Stage<SPAN, ZEROS>::kBytes;
-  static_assert(sizeof(W4Joint) % 16 == 0, "the rings are 16-byte aligned");
+  constexpr int smem = sizeof(W4Joint<NT>) + kW4Warps * kDepth * W4Stage<SPAN, ZEROS>::kBytes;
+  static_assert(sizeof(W4Joint<NT>) % 16 == 0, "the rings are 16-byte aligned");
   static std::atomic<uint64_t> set{0};  // devices whose kernel has its shared memory; setting it twice does no harm
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!((set.load(std::memory_order_relaxed) >> dev) & 1)) {
-    e = cudaFuncSetAttribute(w4_kernel<DT, SPAN, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    e = cudaFuncSetAttribute(w4_kernel<DT, SPAN, ZEROS, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     set.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
   }
-  return launch_pdl(w4_kernel<DT, SPAN, ZEROS>, dim3((unsigned)device_sms()), dim3(kW4Threads), smem, s, a);
+  return launch_pdl(w4_kernel<DT, SPAN, ZEROS, NT>, dim3((unsigned)device_sms()), dim3(kW4Threads), smem, s, a);
+}
+
+template <int DT, int SPAN, bool ZEROS>
+cudaError_t launch_w4_rows(const W4Args& a, cudaStream_t s) {
+  // 8 experts x 8192 outputs x 7168 inputs, units of 8 / of 16 rows: 1 row each 49 / 51 us, 8 rows 52 / 72, 9 rows 93 / 73,
+  // 16 rows 96 / 75, 32 rows 193 / 165.  The host knows the rows of all experts together, not of each: units of 16 where
+  // an expert has more than 8 on average.
+  return a.rows > 8 * (int64_t)a.E ? launch_w4<DT, SPAN, ZEROS, 2>(a, s) : launch_w4<DT, SPAN, ZEROS, 1>(a, s);
 }
 
 template <int DT, bool ZEROS>
 cudaError_t launch_w4_span(const W4Args& a, int group, cudaStream_t s) {
-  if (group % 128 == 0) return launch_w4<DT, 4, ZEROS>(a, s);
-  if (group % 64 == 0) return launch_w4<DT, 2, ZEROS>(a, s);
-  return launch_w4<DT, 1, ZEROS>(a, s);
+  if (group % 128 == 0) return launch_w4_rows<DT, 4, ZEROS>(a, s);
+  if (group % 64 == 0) return launch_w4_rows<DT, 2, ZEROS>(a, s);
+  return launch_w4_rows<DT, 1, ZEROS>(a, s);
 }
 
 }  // namespace

@@ -88,7 +88,8 @@ def expert_matvec_w4(x: torch.Tensor, weights: W4Weights, offsets: Optional[torc
     device tensor as ``route_dispatch`` and ``sort_tokens`` return it, or None for one matrix that every row goes
     through.  Rows that no expert has become zero.  Products are added in fp32 and rounded once.
 
-    Meant for few rows per expert (the weights are read once per eight rows of an expert); right for any number.  For
+    Meant for few rows per expert (the weights of an expert are read once per eight of its rows, or sixteen where
+    there are more than eight per expert on average); right for any number.  For
     inference: a row that requires a gradient is refused.
     """
     if not isinstance(weights, W4Weights):

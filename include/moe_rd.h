@@ -478,8 +478,8 @@ int moe_rd_routing_weights_backward(int64_t T, int32_t E, int32_t K, int32_t sco
  * NULL: one expert (E = 1) that has every row.  Rows before offsets[0] and from
  * offsets[E] on become zero (all rows, where offsets decrease or leave [0, rows]).  The products of a group are added in fp32 and
  * scaled in fp32; the result is rounded once.  Every weight of an expert that has
- * rows is read once per eight of its rows, so the call is meant for few rows per
- * expert; it is right for any number.
+ * rows is read once per eight of its rows (sixteen, where rows > 8 E), so the call is
+ * meant for few rows per expert; it is right for any number.
  * K % group == 0, group % 32 == 0, K <= 2^20; at most 2^31
  * tiles of 32 outputs x 128 inputs x 8 rows (MOE_RD_E_TOO_LARGE); x, weight, scales and
  * zeros 16-byte aligned.  The weights are laid

@@ -50,6 +50,12 @@ CASES = [
     (256, 48, 384, 128, "bf16", False, [0] * 100 + [1] * 3 + [0] * 152 + [2]),
     (3, 64, 7168, 128, "bf16", False, [1, 1, 1]),
     (2, 16, 128, 32, "bf16", False, [0, 0]),
+    # more than eight rows per expert on average: units of sixteen rows
+    (1, 70, 4128, 32, "bf16", True, [16]),
+    (1, 33, 384, 64, "fp16", False, [9]),
+    (1, 200, 1056, 96, "fp16", True, [17]),
+    (3, 64, 2048, 128, "bf16", False, [33, 0, 8]),
+    (2, 4096, 256, 256, "bf16", True, [1, 40]),
 ]
 
 
