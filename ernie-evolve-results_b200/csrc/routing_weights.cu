@@ -28,7 +28,6 @@ int device_sms();
 namespace {
 
 constexpr int kRwThreads = 256;
-constexpr int kRwWarps = kRwThreads / 32;
 
 struct RwArgs {
   const float* logits;
