@@ -141,7 +141,8 @@ extern "C" int moe_rd_unsort_tokens_backward(int64_t T, int32_t H, int32_t K, in
                                              float* grad_weights, void* stream) {
   const int rc = check_rows(T, H, K, dtype, y_rows);
   if (rc != MOE_RD_OK) return rc;
-  if (grad_y == nullptr && grad_weights == nullptr) return MOE_RD_E_NULL;
+  if (grad_y == nullptr && grad_weights == nullptr)  // of an empty batch or of no rows there is nothing to write
+    return T > 0 && y_rows > 0 ? MOE_RD_E_NULL : MOE_RD_OK;
   if (T > 0 && (grad_out == nullptr || inverse_perm == nullptr ||
                 (grad_weights != nullptr && y == nullptr && y_rows > 0)))
     return MOE_RD_E_NULL;

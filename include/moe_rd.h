@@ -435,7 +435,8 @@ int moe_rd_unsort_tokens(int64_t T, int32_t H, int32_t K, int32_t dtype, const v
  *   grad_y[inverse_perm[t,k],:] = weights[t,k] * grad_out[t,:]     (one rounding)
  *   grad_weights[t,k] = sum_h grad_out[t,h] * y[inverse_perm[t,k],h]   (fp32, in
  *                       a fixed order; 0 for a pair without a row)
- * (the gradient of `shared` is grad_out itself).  Either output may be NULL; y is
+ * (the gradient of `shared` is grad_out itself).  Either output may be NULL (both
+ * only where T or y_rows is 0, and then nothing is done); y is
  * read for grad_weights only.  Every row index may occur once at most, as in what
  * moe_rd_sort_tokens and moe_rd_route_dispatch return.  grad_y is written whole:
  * n_rows is a DEVICE int32 (offsets[E]) from which on the rows of y are nobody's

@@ -485,3 +485,17 @@ def test_two_threads_on_two_streams():
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("T,R", [(0, 0), (0, 5), (3, 0)])
+@pytest.mark.parametrize("rows,weights", [(True, True), (True, False), (False, True)])
+def test_gradient_of_an_empty_batch_or_of_no_rows(T, R, rows, weights):
+    grad, y = torch.ones(T, 64, device="cuda"), torch.ones(R, 64, device="cuda")
+    inv, w = torch.full((T, 2), -1, dtype=torch.int32, device="cuda"), torch.ones(T, 2, device="cuda")
+    g = moe_rd.unsort_tokens_backward(grad, y, inv, w, need_rows=rows, need_weights=weights)
+    assert (g.rows is not None) == rows and (g.weights is not None) == weights
+    assert not rows or torch.equal(g.rows, torch.zeros_like(y))
+    assert not weights or torch.equal(g.weights, torch.zeros_like(w))
+    leaf, lw = y.clone().requires_grad_(), w.clone().requires_grad_()
+    moe_rd.unsort_tokens(leaf, inv, lw).sum().backward()
+    assert torch.equal(leaf.grad, torch.zeros_like(y)) and torch.equal(lw.grad, torch.zeros_like(w))
