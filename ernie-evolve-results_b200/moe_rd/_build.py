@@ -1,4 +1,4 @@
-"""Builds libmoe_rd.so in-tree with nvcc for sm_100a (no GPU needed to compile)."""
+"""Builds libmoe_rd.so in-tree with nvcc for sm_100a and _fastcall.so with the host compiler (no GPU needed to compile)."""
 from __future__ import annotations
 
 import os
@@ -11,6 +11,7 @@ PKG = Path(__file__).resolve().parent.parent
 CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 LIB = PKG / "moe_rd" / "libmoe_rd.so"
+FASTCALL = PKG / "moe_rd" / "_fastcall.so"  # Python module: the ordinary call without Python in between
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -26,7 +27,35 @@ def _nvcc() -> str:
     raise RuntimeError("nvcc not found")
 
 
+def build_fastcall(force: bool = False) -> Path:
+    """csrc/fastcall.cpp against the headers of the installed torch and Python."""
+    src = CSRC / "fastcall.cpp"
+    if not force and FASTCALL.exists() and all(FASTCALL.stat().st_mtime >= d.stat().st_mtime for d in (src, INCLUDE / "moe_rd.h")):
+        return FASTCALL
+    import sysconfig
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    cxx = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else "g++"
+    include = [INCLUDE, sysconfig.get_paths()["include"], root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
+               Path(_nvcc()).resolve().parent.parent / "include"]
+    cmd = [cxx, "-O2", "-Wall", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{i}" for i in include], str(src), "-o", str(FASTCALL), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src.name}:\n{r.stdout}\n{r.stderr}")
+    return FASTCALL
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
+    with ThreadPoolExecutor(max_workers=1) as ex:  # beside nvcc
+        fastcall = ex.submit(build_fastcall, force)
+        lib = build_library(force, verbose)
+        fastcall.result()
+    return lib
+
+
+def build_library(force: bool = False, verbose: bool = False) -> Path:
     srcs = sorted(CSRC.glob("*.cu"))
     deps = srcs + sorted(CSRC.glob("*.cuh")) + [INCLUDE / "moe_rd.h"]
     if not force and LIB.exists() and all(LIB.stat().st_mtime >= d.stat().st_mtime for d in deps):

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import warnings
 from pathlib import Path
 
 import torch
@@ -74,8 +75,31 @@ class MoeRdError(RuntimeError):
 _lib = None
 
 
+class _NotLoaded:
+    """Stands for csrc/fastcall.cpp until the library is loaded, or where it is not built: no call is taken over."""
+
+    def __getattr__(self, name):
+        return lambda *args: False
+
+
+fast = _NotLoaded()
+FAST_ENTRIES = ("moe_rd_sort_workspace_bytes", "moe_rd_sort_tokens", "moe_rd_unsort_tokens", "moe_rd_unsort_tokens_backward",
+                "moe_rd_routing_weights", "moe_rd_routing_weights_backward", "moe_rd_expert_matvec_w4")
+
+
+def _load_fast(L: ctypes.CDLL):
+    try:
+        from . import _fastcall
+    except ImportError as e:  # the calls still run, from Python
+        if (_LIB_PATH.parent / "_fastcall.so").exists():
+            warnings.warn(f"moe_rd: _fastcall.so does not load with this torch, rebuild it with `python -m moe_rd._build --force`: {e}")
+        return _NotLoaded()
+    _fastcall.bind(*(ctypes.cast(getattr(L, name), ctypes.c_void_p).value for name in FAST_ENTRIES))
+    return _fastcall
+
+
 def lib() -> ctypes.CDLL:
-    global _lib
+    global _lib, fast
     if _lib is None:
         if not _LIB_PATH.exists():
             raise ImportError(
@@ -155,6 +179,7 @@ def lib() -> ctypes.CDLL:
         L.moe_rd_last_cuda_error.restype = ctypes.c_char_p
         L.moe_rd_version.argtypes = []
         L.moe_rd_version.restype = ctypes.c_int
+        fast = _load_fast(L)
         _lib = L
     return _lib
 

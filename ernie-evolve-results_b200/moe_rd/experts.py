@@ -94,6 +94,9 @@ def expert_matvec_w4(x: torch.Tensor, weights: W4Weights, offsets: Optional[torc
     """
     if not isinstance(weights, W4Weights):
         raise TypeError("expert_matvec_w4: weights must come from pack_w4")
+    done = _cabi.fast.expert_matvec_w4(x, weights, offsets, out)
+    if done is not False:
+        return out if done is True else done
     packed, scales, zeros, N, K, group = weights
     dtype = x.dtype
     if dtype is not torch.bfloat16 and dtype is not torch.float16:

@@ -67,6 +67,13 @@ def dense(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     return t, at
 
 
+def packed(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """The same for what the kernels read element by element: indices, weights, logits (no alignment is needed)."""
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t, t.data_ptr()
+
+
 def check_out(name: str, out: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, index: int, inputs, align: int = 1) -> int:
     """``out`` is a buffer the call may write: of this shape and type, contiguous, apart from the inputs ((address, bytes)
     each).  Returns its address."""
@@ -123,7 +130,7 @@ def _check_rows(name: str, rows: torch.Tensor) -> int:
 # --- sort ------------------------------------------------------------------------------------------------------------
 def _sort(index, T, K, H, x, expert_ids, E, capacity, out):
     x, x_at = dense(x if x.dim() == 2 else x.reshape(T, H))
-    ids, ids_at = dense(expert_ids)
+    ids, ids_at = packed(expert_ids)
     R = min(T * K, E * capacity) if capacity else T * K
     dtype = x.dtype
     code = ROW_DTYPE[dtype]
@@ -178,6 +185,9 @@ def sort_tokens(x: torch.Tensor, expert_ids: torch.Tensor, num_experts: int, *, 
     Differentiable in ``x``; the gradient is ``unsort_tokens(grad_rows, inverse_perm)``.  ``out`` takes the result of
     an earlier call of the same sizes and reuses its buffers (not where ``x`` requires a gradient).
     """
+    done = _cabi.fast.sort_tokens(x, expert_ids, num_experts, capacity, out)
+    if done is not False:
+        return out if done is True else SortedTokens(*done)
     H = _check_rows("sort_tokens", x)
     T, K = _check_ids("sort_tokens", expert_ids)
     if x.numel() != T * H:
@@ -213,8 +223,8 @@ def _check_unsort(name, y, inverse_perm, weights, shared):
 
 def _unsort(index, T, K, H, y, inverse_perm, weights, shared, out):
     y, y_at = dense(y if y.dim() == 2 else y.reshape(-1, H))
-    inv, inv_at = dense(inverse_perm)
-    w, w_at = (None, None) if weights is None else dense(weights)
+    inv, inv_at = packed(inverse_perm)
+    w, w_at = (None, None) if weights is None else packed(weights)
     sh, sh_at = (None, None) if shared is None else dense(shared if shared.dim() == 2 else shared.reshape(T, H))
     R = y.shape[0]
     dtype = y.dtype
@@ -273,6 +283,9 @@ def unsort_tokens(y: torch.Tensor, inverse_perm: torch.Tensor, weights: Optional
     written in one pass; without it it is cleared first.  ``out`` takes a [T, H] buffer (not where a gradient is
     required).
     """
+    done = _cabi.fast.unsort_tokens(y, inverse_perm, weights, shared, offsets, out)
+    if done is not False:
+        return out if done is True else done
     T, K, H = _check_unsort("unsort_tokens", y, inverse_perm, weights, shared)
     index = device_index("unsort_tokens", y, inverse_perm, weights, shared, offsets)
     if offsets is not None:
@@ -298,8 +311,8 @@ def _unsort_backward(index, grad_out, y, y_shape, inverse_perm, weights, offsets
         R *= n
     g, g_at = dense(grad_out if grad_out.dim() == 2 else grad_out.reshape(T, H))
     y, y_at = dense(y if y.dim() == 2 else y.reshape(R, H)) if need_w else (None, None)
-    inv, inv_at = dense(inverse_perm)
-    w, w_at = (None, None) if weights is None else dense(weights)
+    inv, inv_at = packed(inverse_perm)
+    w, w_at = (None, None) if weights is None else packed(weights)
     dtype = g.dtype
     end_at = None if offsets is None else offsets.data_ptr() + 4 * (offsets.numel() - 1)
     rows_at = weights_at = None
@@ -334,6 +347,9 @@ def unsort_tokens_backward(grad_out: torch.Tensor, y: torch.Tensor, inverse_perm
     ``grad_out`` itself.  Rows of y that no pair has (with ``offsets``: those from ``offsets[-1]`` on) get a zero
     gradient.  ``out`` takes the result of an earlier call of the same sizes."""
     need_weights = weights is not None if need_weights is None else need_weights
+    done = _cabi.fast.unsort_tokens_backward(grad_out, y, inverse_perm, weights, offsets, need_rows, need_weights, out)
+    if done is not False:
+        return out if done is True else UnsortGradients(*done)
     _check_unsort("unsort_tokens_backward", y, inverse_perm, weights, grad_out)
     if offsets is not None:
         check_offsets("unsort_tokens_backward", offsets)
@@ -341,6 +357,9 @@ def unsort_tokens_backward(grad_out: torch.Tensor, y: torch.Tensor, inverse_perm
         raise ValueError("unsort_tokens_backward: no gradient is asked for")
     index = device_index("unsort_tokens_backward", grad_out, y, inverse_perm, weights, offsets)
     return _unsort_backward(index, grad_out, y, y.shape, inverse_perm, weights, offsets, need_rows, need_weights, out)
+
+
+_BIAS_USE = {"none": 0, "select": 0, "logit": 1, "select_and_weight": 2}
 
 
 # --- routing weights -------------------------------------------------------------------------------------------------
@@ -366,15 +385,15 @@ def _weights_call(name, entry, index, logits, expert_ids, bias, config, grad, sh
     """One of the two kernels; ``shape`` is that of its result."""
     bias_mode, score_fn, renorm, routed_scale, norm_min = config
     T, E = logits.shape
-    logits, logits_at = dense(logits)
-    ids, ids_at = dense(expert_ids)
+    logits, logits_at = packed(logits)
+    ids, ids_at = packed(expert_ids)
     given = [(logits_at, 4 * T * E), (ids_at, ids.nbytes)]
     bias_at, inputs = None, ()
     if bias is not None:
-        bias, bias_at = dense(bias)
+        bias, bias_at = packed(bias)
         given.append((bias_at, 4 * E))
     if grad is not None:
-        grad, grad_at = dense(grad)
+        grad, grad_at = packed(grad)
         given.append((grad_at, grad.nbytes))
         inputs = (grad_at,)
     if out is None:
@@ -417,6 +436,10 @@ def routing_weights(logits: torch.Tensor, expert_ids: torch.Tensor, bias: Option
     weight 0 and no part in the sum.  Differentiable in ``logits`` (ids and bias are constants): with
     ``logits = x @ gate_weight`` it carries the gradient of the weights to the router.
     """
+    done = _cabi.fast.routing_weights(None, logits, expert_ids, bias, _BIAS_USE.get(bias_mode), SCORE_FN.get(score_fn), renorm, routed_scale,
+                                      norm_min, out)
+    if done is not False:
+        return out if done is True else done
     _check_weights("routing_weights", logits, expert_ids, bias, bias_mode, score_fn)
     index = device_index("routing_weights", logits, expert_ids, bias)
     config = (bias_mode, score_fn, renorm, routed_scale, norm_min)
@@ -436,6 +459,11 @@ def routing_weights_backward(grad_weights: torch.Tensor, logits: torch.Tensor, e
     """Gradient [T, E] fp32 of ``routing_weights`` with respect to the logits, for ``grad_weights`` [T, K] fp32.  Where
     the sum of the chosen scores is below ``norm_min`` it has no part in the gradient; a token without any valid id gets
     zeros."""
+    if grad_weights is not None:
+        done = _cabi.fast.routing_weights(grad_weights, logits, expert_ids, bias, _BIAS_USE.get(bias_mode), SCORE_FN.get(score_fn), renorm,
+                                          routed_scale, norm_min, out)
+        if done is not False:
+            return out if done is True else done
     _check_weights("routing_weights_backward", logits, expert_ids, bias, bias_mode, score_fn)
     if grad_weights.dtype is not torch.float32 or grad_weights.shape != expert_ids.shape:
         raise ValueError("routing_weights_backward: grad_weights must be a float32 tensor like expert_ids")

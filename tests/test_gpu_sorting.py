@@ -499,3 +499,22 @@ def test_gradient_of_an_empty_batch_or_of_no_rows(T, R, rows, weights):
     leaf, lw = y.clone().requires_grad_(), w.clone().requires_grad_()
     moe_rd.unsort_tokens(leaf, inv, lw).sum().backward()
     assert torch.equal(leaf.grad, torch.zeros_like(y)) and torch.equal(lw.grad, torch.zeros_like(w))
+
+
+def test_results_of_the_sort_are_read_where_they_are():
+    """Its parts may start at any multiple of four bytes; passing them on makes no copies."""
+    x, ids = torch.randn(5, 64, device="cuda"), torch.arange(10, dtype=torch.int32, device="cuda").view(5, 2) % 4
+    s, w = moe_rd.sort_tokens(x, ids, 4), torch.rand(11, device="cuda")[1:].view(5, 2)
+    logits = torch.randn(21, device="cuda")[1:].view(5, 4)
+    out = moe_rd.unsort_tokens(s.rows, s.inverse_perm, w)
+    g = moe_rd.unsort_tokens_backward(x, s.rows, s.inverse_perm, w, offsets=s.offsets)
+    r, rg = moe_rd.routing_weights(logits, ids), moe_rd.routing_weights_backward(w, logits, ids)
+    before = torch.cuda.memory_stats()["allocation.all.allocated"]
+    moe_rd.unsort_tokens(s.rows, s.inverse_perm, w, out=out)
+    moe_rd.unsort_tokens_backward(x, s.rows, s.inverse_perm, w, offsets=s.offsets, out=g)
+    moe_rd.routing_weights(logits, ids, out=r)
+    moe_rd.routing_weights_backward(w, logits, ids, out=rg)
+    assert torch.cuda.memory_stats()["allocation.all.allocated"] == before
+    want = sum(w[:, k, None].double() * x.double() for k in range(2))  # every pair's row is its token's
+    assert (out.double() - want).abs().max() <= 4 * 2.0 ** -24 * (2 * w.max() * x.abs().max()).item()
+    assert torch.equal(r, moe_rd.routing_weights(logits.clone(), ids)) and torch.equal(rg, moe_rd.routing_weights_backward(w, logits.clone(), ids))

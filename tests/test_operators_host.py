@@ -165,3 +165,21 @@ def test_capturing_is_refused_where_a_gradient_is_wanted(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(RuntimeError, match="not recorded into a CUDA graph"):
         sorting._not_while_capturing("sort_tokens", "unsort_tokens")
+
+
+def test_the_compiled_calls_leave_everything_else_to_python():
+    from moe_rd import _cabi
+    _cabi.lib()
+    assert not isinstance(_cabi.fast, _cabi._NotLoaded), "moe_rd/_fastcall.so is not built"
+    x, ids, w = torch.zeros(2, 8), torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, 1)
+    f = _cabi.fast
+    for args in ((), (x,), (x, ids, 4, 0, None), (None,) * 5, (x, ids, "4", 0, None), (1, 2, 3, 4, 5)):
+        assert f.sort_tokens(*args) is False
+    for args in ((), (x, ids, w, None, None, None), (None,) * 6):
+        assert f.unsort_tokens(*args) is False
+    for args in ((), (x, x, ids, w, None, True, True, None), (None,) * 8):
+        assert f.unsort_tokens_backward(*args) is False
+    for args in ((), (None, w, ids, None, 0, 0, True, 1.0, 1e-20, None), (None,) * 10):
+        assert f.routing_weights(*args) is False
+    for args in ((), (x, (1, 2, 3, 4, 5, 6), None, None), (x, (None,) * 6, None, None), (None,) * 4):
+        assert f.expert_matvec_w4(*args) is False
