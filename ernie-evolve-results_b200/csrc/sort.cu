@@ -68,7 +68,7 @@ constexpr int kOnceThreads = 256;
 constexpr int kOnceWarps = kOnceThreads / 32;
 constexpr int kOncePairs = 16384;
 // Rows beyond this leave L2 while they are written, and the batch form's even spread over the SMs counts for more than
-// its two launches (times on the device, one kernel / batch form; the host needs 10 / 20 us to enqueue them): K = 8, H =
+// its two launches (times on the device, one kernel / batch form; the host needs 3 / 10 us to enqueue them): K = 8, H =
 // 7168 bf16: 16 tokens 3.0 / 8.2 us, 256 tokens 9.0 / 14.6, 512 tokens (59 MB) 12.9 / 22.3, 2048 tokens (235 MB) 56.7 /
 // 51.2; K = 2, H = 4096: 1024 tokens 5.8 / 9.0, 4096 tokens (67 MB) 23.1 / 21.7.
 constexpr int64_t kOnceBytes = 72 << 20;
