@@ -7,9 +7,9 @@
 // * batch: sort_count_kernel counts the pairs per (tile of 64 tokens, expert) and per (group of 32 tiles, expert);
 //   positions_kernel and scatter_kernel of the routing pipeline (scatter.cu) derive the places from those counts and
 //   copy the rows, each token row read once and stored K times.
-// * up to kOncePairs pairs and kOnceBytes of rows: one kernel.  Every block counts ALL pairs by itself (how many of every
+// * few pairs and few rows (in_one_kernel): one kernel.  Every block counts ALL pairs by itself (how many of every
 //   expert there are, and how many before its own tokens), ranks its own pairs and copies their rows: the counting is
-//   done hundreds of times over, but from L2 and by blocks that would otherwise wait, and one launch does the work of
+//   done once per SM or more, but from L2 and by blocks that would otherwise wait, and one launch does the work of
 //   three.  No workspace.
 // The counts are shared-memory atomics (their order does not matter); with __match_any_sync and one atomic per distinct
 // expert 16384 pairs of 256 experts took 85 us instead of 13.
@@ -64,17 +64,21 @@ sort_count_kernel(const int32_t* __restrict__ ids, int64_t T, int E, int K, int 
   }
 }
 
-constexpr int kOnceThreads = 256;
-constexpr int kOnceWarps = kOnceThreads / 32;
-constexpr int kOncePairs = 16384;
-// Rows beyond this leave L2 while they are written, and the batch form's even spread over the SMs counts for more than
-// its two launches (times on the device, one kernel / batch form; the host needs 3 / 10 us to enqueue them): K = 8, H =
-// 7168 bf16: 16 tokens 3.0 / 8.2 us, 256 tokens 9.0 / 14.6, 512 tokens (59 MB) 12.9 / 22.3, 2048 tokens (235 MB) 56.7 /
-// 51.2; K = 2, H = 4096: 1024 tokens 5.8 / 9.0, 4096 tokens (67 MB) 23.1 / 21.7.
-constexpr int64_t kOnceBytes = 72 << 20;
-constexpr int kOnceBlocksPerSm = 4;
+// The one-kernel form.  Every block counts all pairs, in shared memory: blocks of 1024 threads, one per SM, do that a quarter
+// as often as four of 256 (8192 tokens, K = 2, H = 512: 8.3 us against 11.3; 2048 tokens, K = 8, H = 512: 7.8 / 12.8);
+// of few pairs the copy is all there is, and small blocks start sooner (16 tokens, K = 8, H = 7168: 3.0 with 256 threads,
+// 3.8 with 512, 5.0 with 1024; 256 such tokens 9.2 / 7.5 / 8.6).
+constexpr int kOnceWarpsPerSm = 32;
+constexpr int kSmallPairs = 1024, kMiddlePairs = 4096;  // the last of 256 and of 512 threads
+// Where it ends: its blocks have equal numbers of tokens, whose rows they copy, and the batch form's even spread over the
+// SMs counts for more than its two launches when there is much to copy, or much to count for little (us on the device, one
+// kernel / batch form; the host needs 3 / 10 to enqueue them).  H = 7168, K = 8: 512 tokens 12.7 / 22.5, 1024 (132 MB
+// read and written) 25.9 / 30.2, 2048 (264 MB) 51.3 / 51.3; K = 2, H = 7168, 4096 tokens (176 MB) 34.3 / 33.1; K = 1, H =
+// 4096, 16000 tokens (262 MB) 49.9 / 44.4.  Of 32768 pairs: 1000 tokens, H = 256 9.8 / 21.6, 4096 tokens, H = 512 12.9 /
+// 16.2, 8192 tokens 13.5 / 13.4, 16384 tokens 17.2 / 14.7.
+constexpr int64_t kOnceBytes = 144 << 20;
+constexpr int kOncePairs = 16384, kOnceFewTokens = 4096, kOncePairsOfFewTokens = 32768;
 constexpr int kOwnPairs = 256;  // pairs of a block's tokens
-static_assert(kMaxE <= kOnceThreads && kOwnPairs <= kOnceThreads, "one expert, one pair per thread");
 
 struct OnceArgs {
   const uint4* x;
@@ -90,12 +94,14 @@ struct OnceArgs {
 };
 
 // A unit of the copy: 32 * UV vectors of a row, UV loads in flight per lane.
-template <int UV>
-__global__ void __launch_bounds__(kOnceThreads, kOnceBlocksPerSm) sort_once_kernel(const OnceArgs a) {
+template <int NT, int UV>
+__global__ void __launch_bounds__(NT, 32 * kOnceWarpsPerSm / NT) sort_once_kernel(const OnceArgs a) {
+  static_assert(kMaxE <= NT && kOwnPairs <= NT, "one expert, one pair per thread");
+  constexpr int kWarps = NT / 32;
   __shared__ int s_before[kMaxE], s_after[kMaxE];  // pairs per expert before the block's own, and from them on
-  __shared__ int s_off[kMaxE], s_own[kOwnPairs], s_place[kOwnPairs], s_w[kOnceWarps];
+  __shared__ int s_off[kMaxE], s_own[kOwnPairs], s_place[kOwnPairs], s_w[kMaxE / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  s_before[tid] = s_after[tid] = 0;
+  if (tid < kMaxE) s_before[tid] = s_after[tid] = 0;
   __syncthreads();
   pdl_sync();
   const int t0 = blockIdx.x * a.tokens, ntok = min(a.tokens, a.T - t0);
@@ -103,7 +109,7 @@ __global__ void __launch_bounds__(kOnceThreads, kOnceBlocksPerSm) sort_once_kern
   // the first unit of x is on its way while the places are worked out
   const int upr = (a.nvec + 32 * UV - 1) / (32 * UV);
   const int units = ntok * upr;
-  const int first = blockIdx.y * kOnceWarps + warp, W = gridDim.y * kOnceWarps;
+  const int first = blockIdx.y * kWarps + warp, W = gridDim.y * kWarps;
   const uint4* x = a.x + (size_t)t0 * a.nvec;
   uint4 val[UV];
   auto load = [&](int u) {
@@ -113,19 +119,19 @@ __global__ void __launch_bounds__(kOnceThreads, kOnceBlocksPerSm) sort_once_kern
       if (v + 32 * i < a.nvec) val[i] = __ldg(x + (size_t)t * a.nvec + v + 32 * i);
   };
   if (first < units) load(first);
-  for (int c0 = tid; c0 < P; c0 += 8 * kOnceThreads) {
+  for (int c0 = tid; c0 < P; c0 += 8 * NT) {
     int e[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = c0 + i * kOnceThreads < P ? __ldg(a.ids + c0 + i * kOnceThreads) : -1;
+    for (int i = 0; i < 8; ++i) e[i] = c0 + i * NT < P ? __ldg(a.ids + c0 + i * NT) : -1;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int p = c0 + i * kOnceThreads;
+      const int p = c0 + i * NT;
       if ((unsigned)e[i] < (unsigned)a.E) atomicAdd((p < p0 ? s_before : s_after) + e[i], 1);
       if ((unsigned)(p - p0) < (unsigned)own) s_own[p - p0] = e[i];
     }
   }
   __syncthreads();
-  const int total = s_before[tid] + s_after[tid];
+  const int total = tid < kMaxE ? s_before[tid] + s_after[tid] : 0;
   const int kept = a.capacity > 0 && (int64_t)total > a.capacity ? (int)a.capacity : total;
   int incl = kept;
 #pragma unroll
@@ -133,16 +139,16 @@ __global__ void __launch_bounds__(kOnceThreads, kOnceBlocksPerSm) sort_once_kern
     const int n = __shfl_up_sync(kFull, incl, o);
     if (lane >= o) incl += n;
   }
-  if (lane == 31) s_w[warp] = incl;
+  if (lane == 31 && tid < kMaxE) s_w[warp] = incl;
   __syncthreads();
   int off = incl - kept, all = 0;
 #pragma unroll
-  for (int w = 0; w < kOnceWarps; ++w) {
+  for (int w = 0; w < kMaxE / 32; ++w) {
     const int v = s_w[w];
     if (w < warp) off += v;
     all += v;
   }
-  s_off[tid] = off;
+  if (tid < kMaxE) s_off[tid] = off;
   if (blockIdx.x == 0 && blockIdx.y == 0) {
     if (tid < a.E) {
       a.offsets[tid] = off;
@@ -181,8 +187,8 @@ __global__ void __launch_bounds__(kOnceThreads, kOnceBlocksPerSm) sort_once_kern
   }
   // rows of nobody
   const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, blocks = (int64_t)gridDim.x * gridDim.y;
-  for (int64_t r = (int64_t)all + block * kOnceThreads + tid; r < a.out_rows; r += blocks * kOnceThreads) a.row_token[r] = -1;
-  for (int64_t k = ((int64_t)all * a.nvec) + block * kOnceThreads + tid; k < a.out_rows * a.nvec; k += blocks * kOnceThreads)
+  for (int64_t r = (int64_t)all + block * NT + tid; r < a.out_rows; r += blocks * NT) a.row_token[r] = -1;
+  for (int64_t k = ((int64_t)all * a.nvec) + block * NT + tid; k < a.out_rows * a.nvec; k += blocks * NT)
     __stcs(a.rows + k, make_uint4(0u, 0u, 0u, 0u));
 }
 
@@ -199,7 +205,26 @@ SortWorkspace carve_sort(int64_t T, int32_t E) {
   return w;
 }
 
-bool in_one_kernel(int64_t T, int32_t H16, int32_t K) { return T * K <= kOncePairs && T * K * H16 * 2 <= kOnceBytes; }
+template <int NT>
+cudaError_t launch_once(OnceArgs& a, cudaStream_t s) {
+  constexpr int kWarps = NT / 32;
+  // as many blocks as are resident at once, each with the same number of tokens (at most kOwnPairs pairs); few tokens share their rows' columns out among blocks
+  const int most = device_sms() * (kOnceWarpsPerSm / kWarps);
+  a.tokens = (a.T + most - 1) / most;
+  while (a.tokens > 1 && a.tokens * a.K > kOwnPairs) --a.tokens;
+  const int bx = (a.T + a.tokens - 1) / a.tokens;
+  const int units = (a.nvec + 31) / 32;
+  int by = (a.tokens * units + kWarps - 1) / kWarps;
+  if (by > most / bx) by = most / bx > 1 ? most / bx : 1;
+  // more units than resident warps: fewer and larger ones
+  const dim3 grid((unsigned)bx, (unsigned)by);
+  return (int64_t)a.T * units > (int64_t)most * kWarps * 2 ? launch_pdl(sort_once_kernel<NT, 4>, grid, dim3(NT), 0, s, a)
+                                                           : launch_pdl(sort_once_kernel<NT, 1>, grid, dim3(NT), 0, s, a);
+}
+
+bool in_one_kernel(int64_t T, int32_t H16, int32_t K) {
+  return T * K <= (T <= kOnceFewTokens ? kOncePairsOfFewTokens : kOncePairs) && T * (K + 1) * H16 * 2 <= kOnceBytes;
+}
 
 int check_experts(int64_t T, int32_t E) {
   if (E < 1 || E > kMaxE) return MOE_RD_E_SHAPE;
@@ -256,19 +281,7 @@ extern "C" int moe_rd_sort_tokens(int64_t T, int32_t H, int32_t E, int32_t K, in
     a.E = E;
     a.K = K;
     a.nvec = H16 / 8;
-    // as many blocks as are resident at once, each with the same number of tokens (at most kOwnPairs pairs: there are
-    // kOncePairs at most); few tokens share their rows' columns out among blocks
-    const int most = device_sms() * kOnceBlocksPerSm;
-    a.tokens = (int)((T + most - 1) / most);
-    while (a.tokens > 1 && a.tokens * K > kOwnPairs) --a.tokens;
-    const int bx = (int)((T + a.tokens - 1) / a.tokens);
-    const int units = (a.nvec + 31) / 32;
-    int by = (a.tokens * units + kOnceWarps - 1) / kOnceWarps;
-    if (by > most / bx) by = most / bx > 1 ? most / bx : 1;
-    // more units than resident warps: fewer and larger ones
-    const dim3 grid((unsigned)bx, (unsigned)by);
-    e = T * units > (int64_t)most * kOnceWarps * 2 ? launch_pdl(sort_once_kernel<4>, grid, dim3(kOnceThreads), 0, s, a)
-                                               : launch_pdl(sort_once_kernel<1>, grid, dim3(kOnceThreads), 0, s, a);
+    e = T * K > kMiddlePairs ? launch_once<1024>(a, s) : T * K > kSmallPairs ? launch_once<512>(a, s) : launch_once<256>(a, s);
     count_launch();
   } else {
     const SortWorkspace w = carve_sort(T, E);

@@ -518,3 +518,22 @@ def test_results_of_the_sort_are_read_where_they_are():
     want = sum(w[:, k, None].double() * x.double() for k in range(2))  # every pair's row is its token's
     assert (out.double() - want).abs().max() <= 4 * 2.0 ** -24 * (2 * w.max() * x.abs().max()).item()
     assert torch.equal(r, moe_rd.routing_weights(logits.clone(), ids)) and torch.equal(rg, moe_rd.routing_weights_backward(w, logits.clone(), ids))
+
+
+@pytest.mark.parametrize("T,K,E,H,dtype,capacity,kind", [
+    (1024, 1, 8, 16, "bf16", 0, "random"),        # the last pairs of the smallest blocks
+    (1025, 1, 8, 16, "bf16", 7, "stray"),
+    (512, 8, 256, 264, "fp16", 0, "padded"),      # of the middle ones
+    (4097, 1, 256, 12, "fp32", 0, "stray"),
+    (1024, 32, 256, 24, "bf16", 0, "random"),     # the last pairs of the one-kernel form, for few tokens
+    (4096, 8, 3, 40, "bf16", 5000, "one expert"),
+    (1025, 32, 256, 24, "bf16", 60, "stray"),     # the first of the batch form
+    (4097, 8, 16, 72, "fp16", 0, "none"),
+    (4097, 4, 16, 72, "fp16", 0, "padded"),
+    (6145, 3, 8, 132, "fp32", 0, "stray"),        # one token into a further group of counting tiles
+    (16385, 1, 2, 16, "bf16", 9000, "random"),
+    (2048, 8, 64, 4096, "bf16", 0, "random"),     # the last bytes of the one-kernel form
+    (2049, 8, 64, 4096, "bf16", 0, "random"),
+])
+def test_sort_is_exact_at_the_borders_of_its_forms(T, K, E, H, dtype, capacity, kind):
+    test_sort_is_exact(T, K, E, H, dtype, capacity, kind)
