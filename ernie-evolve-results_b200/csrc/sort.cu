@@ -208,7 +208,8 @@ SortWorkspace carve_sort(int64_t T, int32_t E) {
 template <int NT>
 cudaError_t launch_once(OnceArgs& a, cudaStream_t s) {
   constexpr int kWarps = NT / 32;
-  // as many blocks as are resident at once, each with the same number of tokens (at most kOwnPairs pairs); few tokens share their rows' columns out among blocks
+  // as many blocks as are resident at once, each with the same number of tokens (at most kOwnPairs pairs); few tokens
+  // share their rows' columns out among blocks
   const int most = device_sms() * (kOnceWarpsPerSm / kWarps);
   a.tokens = (a.T + most - 1) / most;
   while (a.tokens > 1 && a.tokens * a.K > kOwnPairs) --a.tokens;
