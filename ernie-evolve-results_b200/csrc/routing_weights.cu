@@ -13,12 +13,14 @@
 // amount) and is left out.  1 - s of the sigmoid is exp(-z) s, not a subtraction.
 //
 // Reading logits and writing gradients once is all the memory traffic there is, so HBM should bound a batch; what has to
-// be kept small is the number of instructions per token.  W = 8, 16 or 32 lanes (the fewest that K slots fit in) share a
-// token, so that a warp works on 4, 2 or 1 at a time: the slots, the reductions and the sums over pairs of slots cost a
+// be kept small is the number of instructions per token.  W = 4, 8, 16 or 32 lanes (the fewest that K slots fit in) share a
+// token, so that a warp works on 8, 4, 2 or 1 at a time: the slots, the reductions and the sums over pairs of slots cost a
 // warp the same whether its lanes belong to one token or to four.  The softmax needs every logit of the token (16-byte
 // loads where E and the address allow it), the sigmoid only those of the chosen experts.  The gradient row is put together
 // in shared memory (background -s_e D, then the chosen experts) and stored whole.
-// 32768 tokens, 128 experts, K = 8, softmax: 10.1 us, against 27 us with a warp per token.
+// 32768 tokens, 128 experts, K = 8, softmax: 10.1 us, against 27 us with a warp per token.  Of 4 lanes and 8 (gradient): 32768
+// tokens, 64 experts, K = 4 6.3 / 8.4 us, 16 experts 3.3 / 7.0; 8192 tokens, 64 experts 4.9 / 4.5, which is why few
+// tokens keep 8 there: the logits of a token are then more lanes' work, and the SMs are not full.
 #include "common.cuh"
 
 namespace moe_rd {
@@ -28,6 +30,7 @@ int device_sms();
 namespace {
 
 constexpr int kRwThreads = 256;
+constexpr int kManyTokens = 16384;
 
 struct RwArgs {
   const float* logits;
@@ -257,10 +260,12 @@ template <bool BACKWARD>
 int launch(RwArgs a, int32_t score_fn, void* stream) {
   a.vec = a.E % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.logits) | (BACKWARD ? reinterpret_cast<uintptr_t>(a.out) : 0)) & 15) == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = a.K <= 8 && a.E <= 128 ? launch_wide<8, 16, BACKWARD>(a, score_fn, s)
-                        : a.K <= 8             ? launch_wide<8, 32, BACKWARD>(a, score_fn, s)
-                        : a.K <= 16            ? launch_wide<16, 16, BACKWARD>(a, score_fn, s)
-                                               : launch_wide<32, 8, BACKWARD>(a, score_fn, s);
+  const cudaError_t e = a.K <= 4 && a.E <= 16                     ? launch_wide<4, 4, BACKWARD>(a, score_fn, s)
+                        : a.K <= 4 && a.E <= 64 && a.T > kManyTokens ? launch_wide<4, 16, BACKWARD>(a, score_fn, s)
+                        : a.K <= 8 && a.E <= 128                     ? launch_wide<8, 16, BACKWARD>(a, score_fn, s)
+                        : a.K <= 8                                   ? launch_wide<8, 32, BACKWARD>(a, score_fn, s)
+                        : a.K <= 16                                  ? launch_wide<16, 16, BACKWARD>(a, score_fn, s)
+                                                                     : launch_wide<32, 8, BACKWARD>(a, score_fn, s);
   count_launch();
   if (e != cudaSuccess) set_last_cuda_error(e);
   return e == cudaSuccess ? MOE_RD_OK : MOE_RD_E_CUDA;

@@ -53,9 +53,9 @@ def weights64(logits, ids, bias, score_fn, bias_mode, renorm, scale, norm_min):
 
 def bounds(logits, ids, bias, grad, score_fn, bias_mode, renorm, scale, norm_min):
     """What 32 bits allow, in units of 2^-24.  An exponential's argument is off by up to 20 units (|z - max| <= 20, rounded),
-    expf by 4, so a score by 24, its sum by 24 + 13 (8 + 5 additions) and the quotient by 63 in all; u, S (6 more)
-    and u / S then by 63 + 69 + 2 < 140 relative.  A gradient element is a sum of products of at most
-    s_k, h_k with h_k = (c g_k - c G / S) / S: s_k 63, G 63 + 63 + 8, S twice 69, each operation 1: < 420 of the sum of
+    expf by 4, so a score by 24, its sum by 24 + 35 (at most 32 + 3 additions) and the quotient by 85 in all; u, S (6 more)
+    and u / S then by 85 + 91 + 2 < 180 relative.  A gradient element is a sum of products of at most
+    s_k, h_k with h_k = (c g_k - c G / S) / S: s_k 85, G 85 + 85 + 8, S twice 91, each operation 1: < 560 of the sum of
     the magnitudes of its terms, which no element of the row exceeds by more than what the row's terms sum up to."""
     z = logits.double() if bias_mode != "logit" else logits.double() + bias.double()
     s = torch.softmax(z, 1) if score_fn == "softmax" else torch.sigmoid(z)
@@ -70,7 +70,7 @@ def bounds(logits, ids, bias, grad, score_fn, bias_mode, renorm, scale, norm_min
         h = (g + (g * uk).sum(1, keepdim=True) / m) / m
     else:
         h = g
-    return 140 * 2.0 ** -24, 420 * 2.0 ** -24 * 2 * (sk * h).sum(1, keepdim=True)
+    return 180 * 2.0 ** -24, 560 * 2.0 ** -24 * 2 * (sk * h).sum(1, keepdim=True)
 
 
 @pytest.mark.parametrize("T,E,K,score_fn,bias_mode,renorm,scale,norm_min", CASES)
@@ -172,3 +172,21 @@ def test_sizes_of_nothing_and_graph():
     logits.normal_()
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip([t.clone() for t in res], step()))
+
+
+@pytest.mark.parametrize("T,E,K,score_fn,bias_mode,renorm,scale,norm_min", [
+    (33, 4, 2, "softmax", "none", True, 1.0, 1e-20),
+    (1, 16, 4, "softmax", "logit", False, 2.5, 1e-20),
+    (300, 13, 3, "softmax", "select_and_weight", True, 1.0, 1e-20),
+    (300, 16, 4, "sigmoid", "select", True, 1.0, 1e-20),
+    (20000, 4, 1, "softmax", "none", False, 1.0, 1e-20),
+    (300, 17, 4, "softmax", "none", True, 1.0, 1e-20),
+    (16384, 64, 4, "softmax", "none", True, 1.0, 1e-20),
+    (16385, 64, 4, "softmax", "none", True, 1.0, 1e-20),
+    (16387, 61, 3, "softmax", "logit", False, 0.5, 1e-20),
+    (20001, 60, 4, "softmax", "select_and_weight", True, 2.5, 0.3),
+    (20001, 64, 4, "sigmoid", "select_and_weight", True, 1.0, 1e-20),
+    (16385, 65, 4, "softmax", "none", True, 1.0, 1e-20),
+])
+def test_weights_and_gradient_of_few_slots(T, E, K, score_fn, bias_mode, renorm, scale, norm_min):
+    test_weights_and_gradient(T, E, K, score_fn, bias_mode, renorm, scale, norm_min)
