@@ -20,14 +20,13 @@
 // The copies alone run at 6.7 TB/s (64 experts x 4096 x 7168: 145 us), the kernel at 5.5 (175 us): what bounds it is the
 // integer pipe, 7 instructions for 8 bf16 weights (5 for fp16, 6 % faster).
 //
-// A unit of work is 32 outputs of one expert for up to eight (or 16, see launch_w4_rows) of its rows; its tiles lie one behind the other in memory,
-// and so do the units of an expert.  Only experts that have rows get units: every block lists them from the offsets.  A
-// block gets a run of whole units, and its warps equal shares of the run's tiles, cut anywhere: a warp streams one
-// contiguous stretch of weights, kDepth tiles ahead of its products (cp.async into its own part of shared memory; it
-// waits for nothing but its own copies), writes the units that it has from end to end, and leaves the sums of the
-// cut ones (at most its first and its last) in shared memory, where after a barrier they are added in the warps' order.
-#include <limits.h>
-
+// A unit of work is 32 outputs of one expert for up to eight of its rows (or 16, see launch_w4_rows); its tiles lie one
+// behind the other in memory, and so do the units of an expert.  Only experts that have rows get units: every block lists
+// them from the offsets.  A block gets a run of whole units, and its warps equal shares of the run's tiles, cut anywhere: a
+// warp streams one contiguous stretch of weights, kDepth tiles ahead of its products (cp.async into its own part of
+// shared memory; it waits for nothing but its own copies), writes the units that it has from end to end, and leaves the
+// sums of the cut ones (at most its first and its last) in shared memory, where after a barrier they are added in the
+// warps' order.
 #include <atomic>
 
 #include "row_types.cuh"
