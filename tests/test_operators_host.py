@@ -111,8 +111,9 @@ def test_c_entries_validate_before_any_cuda_call():
 
     def ws(T, H=64, E=256, K=8, dtype=0, to=ctypes.byref(n)):
         return L.moe_rd_sort_workspace_bytes(T, H, E, K, dtype, to)
-    assert ws(1) == 0 and n.value == 0 and ws(2048) == 0 and n.value == 0
-    assert ws(2049) == 0 and n.value == 256 * 4 * 33 + 256 * 4 * 2
+    # one kernel, without a workspace, up to 32768 pairs of 4096 tokens; then tiles of 64 tokens and groups of 32 tiles
+    assert ws(1) == 0 and n.value == 0 and ws(4096) == 0 and n.value == 0
+    assert ws(4097) == 0 and n.value == 256 * 4 * 65 + 256 * 4 * 3
     assert ws(2048, H=7168) == 0 and n.value == 256 * 4 * 32 + 256 * 4 and ws(2 ** 31 - 1, K=1, E=1) == 0
     assert ws(1, E=257) == ws(1, K=33) == ws(2 ** 31, K=1) == ws(1, H=12) == -2 and ws(1, dtype=3) == -6 and ws(1, to=None) == -1
     assert ws(2 ** 30, K=1) == -10      # 2^24 tiles x 256 experts are not counted in 32 bits
