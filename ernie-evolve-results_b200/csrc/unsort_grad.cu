@@ -5,7 +5,14 @@
 // are gathered and the rows of grad_y scattered, each once, whole: HBM bounds it.  1 to 8 warps of a block share a
 // token, by the length of its row; a lane keeps one fp32 sum per slot over its vectors, in ascending order, the lanes
 // are added by a fixed tree and the warps in ascending order, so grad_w does not depend on scheduling.
-// Rows from *n_rows on belong to no pair: they are set to zero at the end, by all blocks.
+// Rows of y that no pair has get a zero gradient.  Without n_rows all of grad_y is cleared first.  With it the rows from
+// *n_rows on are set to zero at the end, by all blocks; among those before it a caller may have taken pairs out of
+// inverse_perm, and which rows that left without one is found by blocks of their own: each reads all of inverse_perm, marks
+// in shared memory which of its rows (r = its number mod their number) a pair has, and clears the others, usually none.
+// That runs beside the tokens: 16 tokens x 7168 bf16, K = 8, 6.1 us with and without, 2048 x 2048 21.0 / 20.1, 8192 x 7168
+// 318 / 315, 32768 x 2048 366 / 363.  It shows where rows are short and many, because such a block reads 262144 pairs in
+// 20 us: 32768 x 512 106 / 95 (all rows cleared beforehand: 134), 8192 x 128 12.6 / 9.4 (12.6), 16384 x 64 23.4 / 17.1 (20).
+// 32, 64 and 128 of them: 8192 x 1024 45.9, 46.5, 48.0, 32768 x 512 108, 106, 112.
 #include "row_types.cuh"
 
 namespace moe_rd {
@@ -17,19 +24,80 @@ namespace {
 constexpr int kGradThreads = 256;
 constexpr int kGradWarps = kGradThreads / 32;
 constexpr int kGradBlocksPerSm = 16;
+constexpr int kMarkBlocks = 64;    // so many blocks at most look for rows without a pair, or four times as many where
+constexpr int kMarkRows = 32768;   // they had more rows than this otherwise, a byte in shared memory each
+constexpr int kMarkLoads = 8;
+constexpr int kShortRowPairs = 65536, kShortRow = 256;  // more pairs of rows of fewer bytes: all rows are cleared beforehand
 
 struct UnsortGradArgs {
   const uint4* grad_out;
   const uint4* y;
   const int32_t* inverse_perm;
   const float* weights;   // or null: every weight is 1
-  const int32_t* n_rows;  // device value, or null: grad_y was cleared before
+  const int32_t* n_rows;  // device value: the rows from there on are nobody's; or null: all of grad_y was cleared before
   uint4* grad_y;          // or null
   float* grad_weights;
   int64_t T, y_rows;
   int nvec, K;
   int warps_per_token;    // 1, 2, 4 or 8
+  int mark_blocks;        // so many blocks, a power of two, clear the rows before *n_rows that have no pair; 0: all are cleared
 };
+
+// *n_rows, or the rows of y where that is less.
+__device__ __forceinline__ int64_t used_rows(const UnsortGradArgs& a) {
+  if (a.n_rows == nullptr) return a.y_rows;
+  const int64_t n = __ldg(a.n_rows);
+  return n < 0 ? 0 : n < a.y_rows ? n : a.y_rows;
+}
+
+__device__ __forceinline__ void clear_row(const UnsortGradArgs& a, int64_t row, int lane) {
+  for (int v = lane; v < a.nvec; v += 32) __stcs(a.grad_y + (size_t)row * a.nvec + v, make_uint4(0u, 0u, 0u, 0u));
+}
+
+// What a block that looks for rows without a pair does: those of the rows r = blockIdx.x mod mark_blocks.
+__device__ __forceinline__ void clear_own_rows(const UnsortGradArgs& a, unsigned char* s_has) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const unsigned block = blockIdx.x, mask = (unsigned)a.mark_blocks - 1u, log = __popc(mask);
+  const unsigned used = (unsigned)used_rows(a);  // needed at the end only
+  auto rows_before = [&](unsigned r) { return block < r ? (r - block + mask) >> log : 0u; };
+  const unsigned rows = rows_before((unsigned)a.y_rows);  // at most kMarkRows
+  for (unsigned i = tid; i < rows; i += kGradThreads) s_has[i] = 0;
+  __syncthreads();
+  // row block + (i << log) -> i; rows of other blocks, and what is no row, -> past the end
+  auto mark = [&](int r) {
+    const unsigned i = __funnelshift_r((unsigned)r - block, (unsigned)r - block, log);
+    if (i < rows) s_has[i] = 1;
+  };
+  const unsigned P = (unsigned)(a.T * a.K);  // below 2^31
+  const unsigned vectors = (reinterpret_cast<uintptr_t>(a.inverse_perm) & 15) == 0 ? P >> 2 : 0u;
+  const int4* inv4 = reinterpret_cast<const int4*>(a.inverse_perm);
+  for (unsigned c = tid; c < vectors; c += kMarkLoads * kGradThreads) {
+    int4 r[kMarkLoads];
+#pragma unroll
+    for (int i = 0; i < kMarkLoads; ++i) r[i] = c + i * kGradThreads < vectors ? __ldg(inv4 + c + i * kGradThreads) : make_int4(-1, -1, -1, -1);
+#pragma unroll
+    for (int i = 0; i < kMarkLoads; ++i) {
+      mark(r[i].x);
+      mark(r[i].y);
+      mark(r[i].z);
+      mark(r[i].w);
+    }
+  }
+  for (unsigned p0 = 4 * vectors + tid; p0 < P; p0 += kMarkLoads * kGradThreads) {
+    int r[kMarkLoads];
+#pragma unroll
+    for (int i = 0; i < kMarkLoads; ++i) r[i] = p0 + i * kGradThreads < P ? __ldg(a.inverse_perm + p0 + i * kGradThreads) : -1;
+#pragma unroll
+    for (int i = 0; i < kMarkLoads; ++i) mark(r[i]);
+  }
+  __syncthreads();
+  const unsigned mine = rows_before(used);
+  for (unsigned i0 = 32 * warp; i0 < mine; i0 += kGradThreads) {
+    const bool without = i0 + lane < mine && s_has[i0 + lane] == 0;
+    for (unsigned m = __ballot_sync(kFull, without); m != 0u; m &= m - 1u)
+      clear_row(a, ((int64_t)(i0 + __ffs(m) - 1) << log) + block, lane);
+  }
+}
 
 // KT slots at a time; NEED_W: grad_weights is wanted (and y is read).  The compiler left alone takes 128 registers for
 // KT = 8, two blocks per SM; with 80 and three blocks 32768 tokens x 2048, K = 8 take 364 us instead of 401, and with four
@@ -38,13 +106,20 @@ template <int DT, int KT, bool NEED_W>
 __global__ void __launch_bounds__(kGradThreads, KT == 8 ? 3 : KT == 4 ? 4 : 0) unsort_grad_kernel(const UnsortGradArgs a) {
   constexpr int NE = RowVec<DT>::N;
   __shared__ float s_part[kGradWarps][KT];
+  extern __shared__ unsigned char s_has[];
   pdl_sync();
+  if (blockIdx.x < a.mark_blocks) {
+    clear_own_rows(a, s_has);
+    return;
+  }
+  const unsigned used = (unsigned)used_rows(a);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int wpt = a.warps_per_token;
   const int sub = warp & (wpt - 1);            // this warp's share of the token
   const int tokens = kGradWarps / wpt;         // tokens of a block at a time
   // every warp of the block makes the same number of trips: the barriers below are for all of them
-  for (int64_t base = (int64_t)blockIdx.x * tokens; base < a.T; base += (int64_t)gridDim.x * tokens) {
+  const int block = blockIdx.x - a.mark_blocks, blocks = gridDim.x - a.mark_blocks;
+  for (int64_t base = (int64_t)block * tokens; base < a.T; base += (int64_t)blocks * tokens) {
     const int64_t t = base + warp / wpt;
     const bool live = t < a.T;
     for (int k0 = 0; k0 < a.K; k0 += KT) {
@@ -58,7 +133,7 @@ __global__ void __launch_bounds__(kGradThreads, KT == 8 ? 3 : KT == 4 ? 4 : 0) u
       }
 #pragma unroll
       for (int k = 0; k < KT; ++k)
-        if ((uint64_t)(int64_t)pos[k] >= (uint64_t)a.y_rows) pos[k] = -1;
+        if ((unsigned)pos[k] >= used) pos[k] = -1;
       if (live) {
         for (int v = sub * 32 + lane; v < a.nvec; v += wpt * 32) {
           const uint4 gv = __ldg(a.grad_out + (size_t)t * a.nvec + v);
@@ -106,23 +181,23 @@ __global__ void __launch_bounds__(kGradThreads, KT == 8 ? 3 : KT == 4 ? 4 : 0) u
       }
     }
   }
-  if (a.grad_y != nullptr && a.n_rows != nullptr) {
-    int64_t n = __ldg(a.n_rows);
-    n = n < 0 ? 0 : n;
+  if (a.grad_y != nullptr && a.mark_blocks > 0) {
+    const int64_t first = (int64_t)block * kGradWarps + warp, step = (int64_t)blocks * kGradWarps;
     const int upr = (a.nvec + 31) >> 5;
-    for (int64_t u = (int64_t)blockIdx.x * kGradWarps + warp; u < (a.y_rows - n) * upr; u += (int64_t)gridDim.x * kGradWarps) {
+    for (int64_t u = first; u < (a.y_rows - used) * upr; u += step) {
       const int64_t r = u / upr;
       const int v = (int)(u - r * upr) * 32 + lane;
-      if (v < a.nvec) __stcs(a.grad_y + (size_t)(n + r) * a.nvec + v, make_uint4(0u, 0u, 0u, 0u));
+      if (v < a.nvec) __stcs(a.grad_y + (size_t)(used + r) * a.nvec + v, make_uint4(0u, 0u, 0u, 0u));
     }
   }
 }
 
 template <int DT, bool NEED_W>
 cudaError_t launch_typed(const UnsortGradArgs& a, dim3 grid, cudaStream_t s) {
-  if (a.K <= 2) return launch_pdl(unsort_grad_kernel<DT, 2, NEED_W>, grid, dim3(kGradThreads), 0, s, a);
-  if (a.K <= 4) return launch_pdl(unsort_grad_kernel<DT, 4, NEED_W>, grid, dim3(kGradThreads), 0, s, a);
-  return launch_pdl(unsort_grad_kernel<DT, 8, NEED_W>, grid, dim3(kGradThreads), 0, s, a);
+  const size_t smem = a.mark_blocks > 0 ? (size_t)((a.y_rows + a.mark_blocks - 1) / a.mark_blocks) : 0;
+  if (a.K <= 2) return launch_pdl(unsort_grad_kernel<DT, 2, NEED_W>, grid, dim3(kGradThreads), smem, s, a);
+  if (a.K <= 4) return launch_pdl(unsort_grad_kernel<DT, 4, NEED_W>, grid, dim3(kGradThreads), smem, s, a);
+  return launch_pdl(unsort_grad_kernel<DT, 8, NEED_W>, grid, dim3(kGradThreads), smem, s, a);
 }
 
 template <int DT>
@@ -151,7 +226,10 @@ extern "C" int moe_rd_unsort_tokens_backward(int64_t T, int32_t H, int32_t K, in
     return MOE_RD_E_ALIGN;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
-  if (grad_y != nullptr && y_rows > 0 && (n_rows == nullptr || T == 0))
+  // rows without a pair: cleared by blocks that look for them, or all rows beforehand
+  const bool clear_rows = grad_y != nullptr && y_rows > 0 && T > 0 && n_rows != nullptr && y_rows <= (int64_t)4 * kMarkBlocks * kMarkRows &&
+                          (T * K <= kShortRowPairs || H * (dtype == MOE_RD_T_F32 ? 4 : 2) >= kShortRow);
+  if (grad_y != nullptr && y_rows > 0 && !clear_rows)
     e = cudaMemsetAsync(grad_y, 0, (size_t)y_rows * H * (dtype == MOE_RD_T_F32 ? 4 : 2), s);
   if (e == cudaSuccess && T > 0) {
     UnsortGradArgs a = {};
@@ -171,7 +249,15 @@ extern "C" int moe_rd_unsort_tokens_backward(int64_t T, int32_t H, int32_t K, in
     const int tokens = kGradWarps / a.warps_per_token;
     const int64_t want = (T + tokens - 1) / tokens;
     const int64_t cap = (int64_t)device_sms() * kGradBlocksPerSm;
-    const dim3 grid((unsigned)(want < cap ? want : cap));
+    dim3 grid((unsigned)(want < cap ? want : cap));  // cap: more than 4 * kMarkBlocks
+    if (clear_rows) {
+      // one for every 32 KB of rows
+      int n = 1;
+      while (2 * n <= kMarkBlocks && 2 * n <= y_rows * a.nvec / 2048) n *= 2;
+      while (n < 4 * kMarkBlocks && (y_rows + n - 1) / n > kMarkRows) n *= 2;
+      grid.x = (unsigned)(want < cap - n ? want : cap - n) + n;  // as many blocks as without them where that is the most
+      a.mark_blocks = n;
+    }
     if (dtype == MOE_RD_T_BF16)
       e = launch_dtype<MOE_RD_T_BF16>(a, grid, s);
     else if (dtype == MOE_RD_T_FP16)

@@ -279,9 +279,9 @@ def unsort_tokens(y: torch.Tensor, inverse_perm: torch.Tensor, weights: Optional
     outside the rows of y is a pair that contributes nothing, whatever its weight); weights: [T, K] fp32, or None for 1;
     shared: T rows like y's, or None.
 
-    Differentiable in ``y``, ``weights`` and ``shared``.  With ``offsets`` (of the same sort) the gradient of ``y`` is
-    written in one pass; without it it is cleared first.  ``out`` takes a [T, H] buffer (not where a gradient is
-    required).
+    Differentiable in ``y``, ``weights`` and ``shared``; rows of ``y`` that no pair has get a zero gradient.  With
+    ``offsets`` (of the same sort: no pair has a row from ``offsets[-1]`` on) the gradient of ``y`` is written in one
+    pass; without it it is cleared first.  ``out`` takes a [T, H] buffer (not where a gradient is required).
     """
     done = _cabi.fast.unsort_tokens(y, inverse_perm, weights, shared, offsets, out)
     if done is not False:
@@ -344,8 +344,8 @@ def unsort_tokens_backward(grad_out: torch.Tensor, y: torch.Tensor, inverse_perm
                            out: Optional[UnsortGradients] = None) -> UnsortGradients:
     """Gradients of ``unsort_tokens`` for ``grad_out`` [T, H]: of the rows of ``y`` (the type of y) and of ``weights``
     (fp32, added in a fixed order; asked for by default where weights are given).  The gradient of ``shared`` is
-    ``grad_out`` itself.  Rows of y that no pair has (with ``offsets``: those from ``offsets[-1]`` on) get a zero
-    gradient.  ``out`` takes the result of an earlier call of the same sizes."""
+    ``grad_out`` itself.  Rows of y that no pair has get a zero gradient, wherever they are.  ``offsets``: as in
+    ``unsort_tokens``.  ``out`` takes the result of an earlier call of the same sizes."""
     need_weights = weights is not None if need_weights is None else need_weights
     done = _cabi.fast.unsort_tokens_backward(grad_out, y, inverse_perm, weights, offsets, need_rows, need_weights, out)
     if done is not False:

@@ -439,8 +439,10 @@ int moe_rd_unsort_tokens(int64_t T, int32_t H, int32_t K, int32_t dtype, const v
  * only where T or y_rows is 0, and then nothing is done); y is
  * read for grad_weights only.  Every row index may occur once at most, as in what
  * moe_rd_sort_tokens and moe_rd_route_dispatch return.  grad_y is written whole:
- * n_rows is a DEVICE int32 (offsets[E]) from which on the rows of y are nobody's
- * and their gradient is zero; with n_rows NULL all of grad_y is cleared first.
+ * rows of y that no pair has, wherever they are, get zeros.  n_rows is a DEVICE
+ * int32 (offsets[E]) from which on the rows of y are nobody's (a pair with such a
+ * row is one without a row); it spares clearing all of grad_y first, as is done
+ * where n_rows is NULL.
  */
 int moe_rd_unsort_tokens_backward(int64_t T, int32_t H, int32_t K, int32_t dtype, const void* grad_out,
                                   const void* y, int64_t y_rows, const int32_t* inverse_perm,

@@ -537,3 +537,63 @@ def test_results_of_the_sort_are_read_where_they_are():
 ])
 def test_sort_is_exact_at_the_borders_of_its_forms(T, K, E, H, dtype, capacity, kind):
     test_sort_is_exact(T, K, E, H, dtype, capacity, kind)
+
+
+@pytest.mark.parametrize("T,K,E,H,dtype,rows", [
+    (1, 2, 4, 8, "bf16", 5),
+    (1, 8, 256, 7168, "bf16", 8),
+    (37, 4, 16, 264, "fp16", 148),
+    (300, 3, 7, 20, "fp32", 2000),          # more rows than pairs
+    (4096, 8, 64, 40, "bf16", 32768),
+    (20000, 2, 8, 136, "fp16", 50001),
+    (30001, 3, 8, 8, "bf16", 32768 * 64 + 1),   # more blocks that look for rows without a pair
+    (3, 2, 4, 8, "bf16", 32768 * 256),          # the last number of rows that they take
+    (30001, 3, 8, 8, "fp16", 32768 * 256 + 1),  # the first that they do not
+])
+@pytest.mark.parametrize("with_offsets", [True, False])
+def test_gradient_of_rows_that_lost_their_pair(T, K, E, H, dtype, rows, with_offsets):
+    """Pairs taken out of inverse_perm after the sort leave rows below offsets[-1] that nobody has: their gradient is zero."""
+    g = torch.Generator().manual_seed(T + K)
+    s = moe_rd.sort_tokens(torch.randn(T, H, generator=g).to(DT[dtype]).cuda(), ids_of(T, K, E, "padded").cuda(), E)
+    inv = s.inverse_perm.clone()
+    inv[torch.rand(T, K, generator=g).cuda() < 0.4] = -1
+    inv[:, 0] = torch.where(inv[:, 0] % 5 == 0, 2 ** 31 - 1, inv[:, 0])   # an index outside the rows is a pair without one
+    y = torch.zeros(rows, H, dtype=DT[dtype], device="cuda")
+    grad = torch.randn(T, H, generator=g).to(DT[dtype]).cuda()
+    has = (inv >= 0) & (inv < rows)
+    offsets = s.offsets if with_offsets else None
+    if with_offsets and T > 100:            # a row from offsets[-1] on is nobody's, whatever a pair says
+        offsets = offsets - 13
+        has &= inv < offsets[-1]
+    want = torch.zeros_like(y)
+    want[inv[has].long()] = grad[:, None, :].expand(T, K, H)[has]      # weights of 1: not rounded
+    out = moe_rd.UnsortGradients(torch.full_like(y, float("nan")), None)
+    got = moe_rd.unsort_tokens_backward(grad, y, inv, offsets=offsets, out=out)
+    assert got is out and torch.equal(got.rows, want)
+    ones = torch.ones(T, K, device="cuda")
+    both = moe_rd.unsort_tokens_backward(grad, y, inv, ones, offsets=offsets,
+                                         out=moe_rd.UnsortGradients(torch.full_like(y, float("nan")), torch.full_like(ones, float("nan"))))
+    assert torch.equal(both.rows, want) and torch.equal(both.weights, torch.zeros_like(ones))
+    leaf = y.requires_grad_()
+    moe_rd.unsort_tokens(leaf, inv, ones, offsets=offsets).backward(grad)
+    assert torch.equal(leaf.grad, want)
+
+
+def test_gradient_of_rows_without_a_pair_replayed_for_other_places():
+    """A recorded gradient clears the rows of the places that it finds, not of those that it was recorded with."""
+    for T, K, H, more in ((50, 2, 64, 0), (20000, 2, 16, 0), (5000, 2, 4, 32768 * 64), (7, 2, 4, 32768 * 256)):
+        grad, y = torch.randn(T, H, device="cuda"), torch.zeros(T * K + more, H, device="cuda")
+        inv = torch.arange(T * K, dtype=torch.int32, device="cuda").view(T, K)
+        offsets = torch.tensor([0, T * K], dtype=torch.int32, device="cuda")
+        out = moe_rd.unsort_tokens_backward(grad, y, inv, offsets=offsets)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            moe_rd.unsort_tokens_backward(grad, y, inv, offsets=offsets, out=out)
+        for shift in (0, 1, 7):
+            inv.copy_(torch.arange(T * K, dtype=torch.int32, device="cuda").view(T, K).roll(shift) - shift)
+            graph.replay()
+            want = torch.zeros_like(y)
+            has = inv >= 0
+            want[inv[has].long()] = grad[:, None, :].expand(T, K, H)[has]
+            assert torch.equal(out.rows, want)
