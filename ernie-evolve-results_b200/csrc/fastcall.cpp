@@ -1,5 +1,5 @@
 // The ordinary call of the operators of moe_rd.sorting and moe_rd.experts without Python in between: dense, aligned
-// tensors of the right types on the current device, no gradient.  Each function looks at its arguments, calls the C
+// tensors of the right types on the current device, no gradient, no tangent.  Each function looks at its arguments, calls the C
 // entry on the current stream and returns
 //   True           done, results are in `out`;
 //   the results    done, where `out` was None;
@@ -13,6 +13,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -52,7 +53,10 @@ bool dense(const Tensor* t, int device, at::ScalarType type) {
   return packed(t, device, type) && (reinterpret_cast<uintptr_t>(t->const_data_ptr()) & 15) == 0;
 }
 
-bool no_grad(const Tensor* t) { return t == nullptr || !t->requires_grad() || !c10::GradMode::is_enabled(); }
+// Carries a tangent of forward mode that an operation would have to carry on.
+bool dual(const Tensor* t) { return t != nullptr && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t->_fw_grad(0).defined(); }
+
+bool no_grad(const Tensor* t) { return t == nullptr || ((!t->requires_grad() || !c10::GradMode::is_enabled()) && !dual(t)); }
 
 struct Span {
   uintptr_t lo, hi;
@@ -328,7 +332,7 @@ PyObject* routing_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
     double scale, least;
     if (device < 0 || !number(a[4], &use) || !number(a[5], &score_fn) || (a[6] != Py_True && a[6] != Py_False) || !real(a[7], &scale) ||
         !real(a[8], &least) || !packed(z, device, at::kFloat) || !packed(ids, device, at::kInt) || (a[0] != Py_None && !packed(g, device, at::kFloat)) ||
-        (a[3] != Py_None && !packed(b, device, at::kFloat)) || !no_grad(z) || !no_grad(b))
+        (a[3] != Py_None && !packed(b, device, at::kFloat)) || !no_grad(z) || !no_grad(b) || dual(g))
       return refuse();
     if (z->dim() != 2 || ids->dim() != 2 || z->size(0) != ids->size(0) || z->size(1) < 1 || z->size(1) > 256 ||
         ids->size(1) < 1 || ids->size(1) > 32 || (b != nullptr && b->numel() != z->size(1)) ||

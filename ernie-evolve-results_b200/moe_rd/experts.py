@@ -8,7 +8,7 @@ import torch
 
 from . import _cabi
 from ._cabi import ROW_DTYPE
-from .sorting import call, check_offsets, check_out, dense, device_index, wants_grad, written
+from .sorting import call, check_offsets, check_out, dense, device_index, refuse_tangents, wants_grad, written
 
 
 class W4Weights(NamedTuple):
@@ -120,6 +120,7 @@ def expert_matvec_w4(x: torch.Tensor, weights: W4Weights, offsets: Optional[torc
             raise ValueError(f"expert_matvec_w4: offsets must have {E + 1} elements")
     if wants_grad(x, scales):
         raise RuntimeError("expert_matvec_w4 is for inference and has no gradient: pass detached rows")
+    refuse_tangents("expert_matvec_w4", x, scales)
     index = device_index("expert_matvec_w4", x, packed, scales, zeros, offsets)
     x, x_at = dense(x)
     R = x.shape[0]

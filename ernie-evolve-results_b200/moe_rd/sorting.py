@@ -5,13 +5,15 @@ training and for routings that come from elsewhere: ``sort_tokens`` (rows in exp
 ``unsort_tokens`` (the weighted way back) and ``routing_weights`` (the combine weights of chosen experts as a function
 of the logits).  Where an argument requires a gradient, autograd reaches the hand-written backward kernels; the same
 kernels are there as plain functions (``unsort_tokens_backward``, ``routing_weights_backward``; the gradient of the sort
-is ``unsort_tokens`` without weights), which are what a CUDA graph may record.
+is ``unsort_tokens`` without weights), which are what a CUDA graph may record.  There is no forward-mode derivative: tensors
+that carry a tangent are refused.
 """
 from __future__ import annotations
 
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _cabi
 from ._cabi import BIAS_MODES, ROW_DTYPE, SCORE_FN
@@ -100,6 +102,15 @@ def wants_grad(*tensors: Optional[torch.Tensor]) -> bool:
             if t is not None and t.requires_grad:
                 return True
     return False
+
+
+def refuse_tangents(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Forward mode: a tangent would be dropped without a word (an ``autograd.Function`` of the caller, whose ``jvp`` carries
+    it on, calls with forward mode off)."""
+    if torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if t is not None and unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"moe_rd.{name} has no forward-mode derivative: pass tensors without a tangent")
 
 
 def _not_while_capturing(name: str, instead: str) -> None:
@@ -195,6 +206,7 @@ def sort_tokens(x: torch.Tensor, expert_ids: torch.Tensor, num_experts: int, *, 
     if num_experts < 1 or capacity < 0:
         raise ValueError("sort_tokens: num_experts must be positive and capacity not negative")
     num_experts, capacity = int(num_experts), int(capacity)
+    refuse_tangents("sort_tokens", x)
     index = device_index("sort_tokens", x, expert_ids)
     if not wants_grad(x):
         return _sort(index, T, K, H, x, expert_ids, num_experts, capacity, out)
@@ -287,6 +299,7 @@ def unsort_tokens(y: torch.Tensor, inverse_perm: torch.Tensor, weights: Optional
     if done is not False:
         return out if done is True else done
     T, K, H = _check_unsort("unsort_tokens", y, inverse_perm, weights, shared)
+    refuse_tangents("unsort_tokens", y, weights, shared)
     index = device_index("unsort_tokens", y, inverse_perm, weights, shared, offsets)
     if offsets is not None:
         check_offsets("unsort_tokens", offsets)
@@ -351,6 +364,7 @@ def unsort_tokens_backward(grad_out: torch.Tensor, y: torch.Tensor, inverse_perm
     if done is not False:
         return out if done is True else UnsortGradients(*done)
     _check_unsort("unsort_tokens_backward", y, inverse_perm, weights, grad_out)
+    refuse_tangents("unsort_tokens_backward", grad_out, y, weights)
     if offsets is not None:
         check_offsets("unsort_tokens_backward", offsets)
     if not (need_rows or need_weights):
@@ -441,6 +455,7 @@ def routing_weights(logits: torch.Tensor, expert_ids: torch.Tensor, bias: Option
     if done is not False:
         return out if done is True else done
     _check_weights("routing_weights", logits, expert_ids, bias, bias_mode, score_fn)
+    refuse_tangents("routing_weights", logits, bias)
     index = device_index("routing_weights", logits, expert_ids, bias)
     config = (bias_mode, score_fn, renorm, routed_scale, norm_min)
     if wants_grad(logits):
@@ -467,6 +482,7 @@ def routing_weights_backward(grad_weights: torch.Tensor, logits: torch.Tensor, e
     _check_weights("routing_weights_backward", logits, expert_ids, bias, bias_mode, score_fn)
     if grad_weights.dtype is not torch.float32 or grad_weights.shape != expert_ids.shape:
         raise ValueError("routing_weights_backward: grad_weights must be a float32 tensor like expert_ids")
+    refuse_tangents("routing_weights_backward", grad_weights, logits, bias)
     index = device_index("routing_weights_backward", logits, grad_weights, expert_ids, bias)
     return _weights_call("routing_weights_backward", _cabi.lib().moe_rd_routing_weights_backward, index, logits, expert_ids, bias,
                          (bias_mode, score_fn, renorm, routed_scale, norm_min), grad_weights, logits.shape, out)

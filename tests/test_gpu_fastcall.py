@@ -240,3 +240,46 @@ def test_from_several_threads(recorder):
     for t in threads:
         t.join()
     assert not failed
+
+
+@pytest.mark.parametrize("fast", [True, False])
+def test_tangents_of_forward_mode_are_refused(recorder, monkeypatch, fast):
+    """They would be dropped; a Function of the caller's that carries them on itself may call."""
+    import torch.autograd.forward_ad as fwad
+    if not fast:
+        monkeypatch.setattr(_cabi, "fast", _cabi._NotLoaded())
+    x, ids, w, logits, bias, grad, grad_w = inputs(dtype=torch.float32)
+    s = moe_rd.sort_tokens(x, ids, 16)
+    half, p = x.bfloat16(), w4(E=1)
+    scales = p.scales
+
+    class Sorted(torch.autograd.Function):
+        @staticmethod
+        def forward(x, ids):
+            return moe_rd.sort_tokens(x, ids, 16).rows
+
+        @staticmethod
+        def setup_context(ctx, inputs, output):
+            ctx.ids = inputs[1]
+
+        @staticmethod
+        def jvp(ctx, tangent, _):
+            return moe_rd.sort_tokens(tangent, ctx.ids, 16).rows
+
+    with fwad.dual_level():
+        dual = lambda t: fwad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: moe_rd.sort_tokens(dual(x), ids, 16), lambda: moe_rd.sort_tokens(dual(x), ids, 16, out=s),
+                     lambda: moe_rd.unsort_tokens(dual(s.rows), s.inverse_perm, w), lambda: moe_rd.unsort_tokens(s.rows, s.inverse_perm, dual(w)),
+                     lambda: moe_rd.unsort_tokens(s.rows, s.inverse_perm, w, dual(x)), lambda: moe_rd.unsort_tokens_backward(dual(grad), s.rows, s.inverse_perm, w),
+                     lambda: moe_rd.unsort_tokens_backward(grad, s.rows, s.inverse_perm, dual(w)), lambda: moe_rd.routing_weights(dual(logits), ids),
+                     lambda: moe_rd.routing_weights(dual(logits.clone().requires_grad_()), ids),
+                     lambda: moe_rd.routing_weights(logits, ids, dual(bias), bias_mode="logit"), lambda: moe_rd.routing_weights_backward(dual(grad_w), logits, ids),
+                     lambda: moe_rd.routing_weights_backward(grad_w, dual(logits), ids), lambda: moe_rd.expert_matvec_w4(dual(half), p),
+                     lambda: moe_rd.expert_matvec_w4(half, p._replace(scales=dual(scales)))):
+            recorder.taken.clear()
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            assert not any(recorder.taken)
+        same(moe_rd.sort_tokens(x, ids, 16), s)                       # a level that is open changes nothing for others
+        primal, tangent = fwad.unpack_dual(Sorted.apply(dual(x), ids))
+        assert torch.equal(primal, s.rows) and torch.equal(tangent, moe_rd.sort_tokens(torch.ones_like(x), ids, 16).rows)

@@ -184,3 +184,23 @@ def test_the_compiled_calls_leave_everything_else_to_python():
         assert f.routing_weights(*args) is False
     for args in ((), (x, (1, 2, 3, 4, 5, 6), None, None), (x, (None,) * 6, None, None), (None,) * 4):
         assert f.expert_matvec_w4(*args) is False
+
+
+def test_tangents_of_forward_mode_are_refused():
+    import torch.autograd.forward_ad as fwad
+    rows, ids, w = x(4, 64), torch.zeros(4, 2, dtype=I32), torch.zeros(4, 2)
+    y, logits, bias = x(8, 64), torch.zeros(4, 8), torch.zeros(8)
+    p = moe_rd.pack_w4(torch.zeros(40, 32, dtype=torch.uint8), torch.ones(40, 2).bfloat16())
+    with fwad.dual_level():
+        dual = lambda t: fwad.make_dual(t, torch.ones_like(t))
+        calls = (lambda: moe_rd.sort_tokens(dual(rows), ids, 8), lambda: moe_rd.unsort_tokens(dual(y), ids), lambda: moe_rd.unsort_tokens(y, ids, dual(w)),
+                 lambda: moe_rd.unsort_tokens(y, ids, w, dual(rows)), lambda: moe_rd.unsort_tokens_backward(dual(rows), y, ids, w),
+                 lambda: moe_rd.unsort_tokens_backward(rows, dual(y), ids, w), lambda: moe_rd.unsort_tokens_backward(rows, y, ids, dual(w)),
+                 lambda: moe_rd.routing_weights(dual(logits), ids), lambda: moe_rd.routing_weights(logits, ids, dual(bias)),
+                 lambda: moe_rd.routing_weights_backward(dual(w), logits, ids), lambda: moe_rd.routing_weights_backward(w, dual(logits), ids),
+                 lambda: moe_rd.expert_matvec_w4(dual(rows), p))
+        for call in calls:
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
