@@ -193,12 +193,13 @@ PyObject* sort_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
     {
       WithoutLock lock;
       if (!given) {
-        const Tensor ints = at::empty({2 * E + 1 + all + R}, ids->options());
+        // parts of one buffer would share its version: a change of the counts would look like one of the places, which
+        // a graph may have saved
         made[0] = at::empty({R, H}, x->options());
-        made[1] = ints.narrow(0, 0, E + 1);
-        made[2] = ints.narrow(0, E + 1, all).view({T, K});
-        made[3] = ints.narrow(0, E + 1 + all, R);
-        made[4] = ints.narrow(0, E + 1 + all + R, E);
+        made[1] = at::empty({E + 1}, ids->options());
+        made[2] = at::empty({T, K}, ids->options());
+        made[3] = at::empty({R}, ids->options());
+        made[4] = at::empty({E}, ids->options());
         for (int i = 0; i < 5; ++i) out[i] = &made[i];
       }
       size_t bytes = 0;

@@ -146,9 +146,10 @@ def _sort(index, T, K, H, x, expert_ids, E, capacity, out):
     dtype = x.dtype
     code = ROW_DTYPE[dtype]
     if out is None:
-        ints = torch.empty(2 * E + 1 + T * K + R, dtype=torch.int32, device=x.device)
-        offsets, inv, row_token, counts = ints.split((E + 1, T * K, R, E))
-        result = SortedTokens(torch.empty((R, H), dtype=dtype, device=x.device), offsets, inv.view(T, K), row_token, counts)
+        # parts of one buffer would share its version: a change of the counts would look like one of the places, which a
+        # graph may have saved
+        result = SortedTokens(torch.empty((R, H), dtype=dtype, device=x.device),
+                              *(torch.empty(n, dtype=torch.int32, device=x.device) for n in ((E + 1,), (T, K), (R,), (E,))))
         at = [t.data_ptr() for t in result]
     else:
         result = out

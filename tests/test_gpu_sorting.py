@@ -597,3 +597,25 @@ def test_gradient_of_rows_without_a_pair_replayed_for_other_places():
             has = inv >= 0
             want[inv[has].long()] = grad[:, None, :].expand(T, K, H)[has]
             assert torch.equal(out.rows, want)
+
+
+@pytest.mark.parametrize("leaf", [True, False])
+def test_what_the_sort_returns_may_be_changed_part_by_part(leaf):
+    """Counts and tokens of rows are the caller's to change in place; the places, which the graph has saved, are not."""
+    for part in ("row_token", "counts", "inverse_perm"):
+        x = torch.randn(50, 64, device="cuda", requires_grad=leaf)
+        ids = ids_of(50, 2, 8, "padded").cuda()
+        s = moe_rd.sort_tokens(x, ids, 8)
+        y = s.rows if leaf else s.rows.requires_grad_()
+        places = [t.clone() for t in (s.inverse_perm, s.offsets)]
+        out = moe_rd.unsort_tokens(y, s.inverse_perm, offsets=s.offsets)
+        getattr(s, part).add_(1)
+        if part == "inverse_perm":
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                out.sum().backward()
+            continue
+        out.sum().backward()
+        assert torch.equal(s.inverse_perm, places[0]) and torch.equal(s.offsets, places[1])
+        n = (ids >= 0).sum(1, keepdim=True).float()
+        want = n.expand(50, 64) if leaf else (torch.arange(100, device="cuda") < s.offsets[-1])[:, None].float().expand(100, 64)
+        assert torch.equal(x.grad if leaf else y.grad, want)
