@@ -41,11 +41,11 @@ constexpr Py_ssize_t kEntries = sizeof(Entries) / sizeof(void*);
 
 const Tensor* tensor(PyObject* o) { return THPVariable_CheckExact(o) ? &THPVariable_Unpack(o) : nullptr; }
 
-// Dense, on the device, of the type.
+// Dense, on the device, of the type, in memory as it is (not the imaginary part of a conjugate, whose sign is still to change).
 bool packed(const Tensor* t, int device, at::ScalarType type) {
   return t != nullptr && t->defined() && t->is_cuda() && t->get_device() == device && t->layout() == at::kStrided &&
          t->unsafeGetTensorImpl()->has_storage() && t->is_contiguous() &&
-         t->scalar_type() == type;
+         t->scalar_type() == type && !t->is_neg();
 }
 
 // The same with an address that is a multiple of 16: what the kernels read in vectors.
@@ -70,7 +70,7 @@ bool writable(const Tensor* t, int device, at::ScalarType type, at::IntArrayRef 
               bool aligned = true) {
   if (t == nullptr || !t->defined() || !t->is_cuda() || t->get_device() != device || t->layout() != at::kStrided ||
       !t->unsafeGetTensorImpl()->has_storage() || t->scalar_type() != type || t->sizes() != shape || !t->is_contiguous() ||
-      t->requires_grad() ||
+      t->requires_grad() || t->is_neg() ||
       (aligned && (reinterpret_cast<uintptr_t>(t->const_data_ptr()) & 15) != 0))
     return false;
   const Span mine(t);

@@ -60,6 +60,7 @@ def call(index: int, entry, *args) -> None:
 
 def dense(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """The tensor, or a copy of it, contiguous and 16-byte aligned (a view may start anywhere), and its address."""
+    t = t.resolve_neg()
     if not t.is_contiguous():
         t = t.contiguous()
     at = t.data_ptr()
@@ -71,6 +72,7 @@ def dense(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
 
 def packed(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """The same for what the kernels read element by element: indices, weights, logits (no alignment is needed)."""
+    t = t.resolve_neg()
     if not t.is_contiguous():
         t = t.contiguous()
     return t, t.data_ptr()
@@ -79,7 +81,7 @@ def packed(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
 def check_out(name: str, out: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, index: int, inputs, align: int = 1) -> int:
     """``out`` is a buffer the call may write: of this shape and type, contiguous, apart from the inputs ((address, bytes)
     each).  Returns its address."""
-    if out.shape != shape or out.dtype is not dtype or out.get_device() != index or not out.is_contiguous() or out.requires_grad:
+    if out.shape != shape or out.dtype is not dtype or out.get_device() != index or not out.is_contiguous() or out.requires_grad or out.is_neg():
         raise ValueError(f"{name}: out must be a contiguous {dtype} tensor of shape {tuple(shape)} on cuda:{index} that needs no gradient")
     lo = out.data_ptr()
     if lo % align:

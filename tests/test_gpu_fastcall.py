@@ -283,3 +283,26 @@ def test_tangents_of_forward_mode_are_refused(recorder, monkeypatch, fast):
         same(moe_rd.sort_tokens(x, ids, 16), s)                       # a level that is open changes nothing for others
         primal, tangent = fwad.unpack_dual(Sorted.apply(dual(x), ids))
         assert torch.equal(primal, s.rows) and torch.equal(tangent, moe_rd.sort_tokens(torch.ones_like(x), ids, 16).rows)
+
+
+@pytest.mark.parametrize("fast", [True, False])
+def test_a_sign_that_is_still_to_change(recorder, monkeypatch, fast):
+    """The imaginary part of a conjugate is a view whose numbers in memory have the other sign."""
+    if not fast:
+        monkeypatch.setattr(_cabi, "fast", _cabi._NotLoaded())
+    g = torch.Generator().manual_seed(0)
+    of = lambda *shape: torch.randn(*shape, generator=g, dtype=torch.complex64).cuda().conj().imag
+    rows, w, logits, ids = of(1, 64), of(1, 1), of(1, 1), torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    assert all(t.is_neg() for t in (rows, w, logits)) and w.is_contiguous()
+    plain = lambda t: t.resolve_neg().contiguous()
+    inv = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    same(moe_rd.sort_tokens(rows, ids, 1), moe_rd.sort_tokens(plain(rows), ids, 1))
+    got = moe_rd.unsort_tokens(rows, inv, w, rows)
+    same(got, moe_rd.unsort_tokens(plain(rows), inv, plain(w), plain(rows)))
+    assert (got.double() - (1 + plain(w).double()) * plain(rows).double()).abs().max() <= 2.0 ** -22 * ((1 + w.abs()) * rows.abs().max()).item()
+    same(moe_rd.unsort_tokens_backward(rows, rows, inv, w), moe_rd.unsort_tokens_backward(plain(rows), plain(rows), inv, plain(w)))
+    config = dict(score_fn="sigmoid", renorm=False)
+    same(moe_rd.routing_weights(logits, ids, w, bias_mode="logit", **config), moe_rd.routing_weights(plain(logits), ids, plain(w), bias_mode="logit", **config))
+    same(moe_rd.routing_weights_backward(w, logits, ids, **config), moe_rd.routing_weights_backward(plain(w), plain(logits), ids, **config))
+    with pytest.raises(ValueError, match="out must be"):
+        moe_rd.routing_weights(plain(logits), ids, out=of(1, 1))
