@@ -10,6 +10,9 @@
 // smallest calls take the GPU 3 to 6 us, so that a decode step pays for the host in every one of them.
 //
 // The C entries come as addresses from the Python side, which has loaded the library (bind).
+//
+// The objects of torch and Python are read in place, so a module fits the versions that it was compiled for and no others:
+// it carries their names (BUILT_FOR), and is loaded only where they are the running ones.
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -435,4 +438,8 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_fastcall", nullptr, -1, g_metho
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__fastcall(void) { return PyModule_Create(&g_module); }
+PyMODINIT_FUNC PyInit__fastcall(void) {
+  PyObject* m = PyModule_Create(&g_module);
+  if (m != nullptr && PyModule_AddStringConstant(m, "BUILT_FOR", MOE_RD_BUILT_FOR) != 0) Py_CLEAR(m);
+  return m;
+}

@@ -27,10 +27,23 @@ def _nvcc() -> str:
     raise RuntimeError("nvcc not found")
 
 
+def fastcall_stamp() -> str:
+    """What _fastcall.so is compiled for: it reads torch's and Python's objects in place, as their headers lay them out."""
+    import sysconfig
+    import torch
+    return f"moe_rd fastcall for torch {torch.__version__} {torch.version.git_version}, {sysconfig.get_config_var('SOABI')}"
+
+
+def fastcall_fits() -> bool:
+    """Whether the _fastcall.so that is there was compiled for the torch and Python that run (seen without loading it)."""
+    return fastcall_stamp().encode() + b"\0" in FASTCALL.read_bytes()
+
+
 def build_fastcall(force: bool = False) -> Path:
     """csrc/fastcall.cpp against the headers of the installed torch and Python."""
     src = CSRC / "fastcall.cpp"
-    if not force and FASTCALL.exists() and all(FASTCALL.stat().st_mtime >= d.stat().st_mtime for d in (src, INCLUDE / "moe_rd.h")):
+    if (not force and FASTCALL.exists() and all(FASTCALL.stat().st_mtime >= d.stat().st_mtime for d in (src, INCLUDE / "moe_rd.h"))
+            and fastcall_fits()):
         return FASTCALL
     import sysconfig
     import torch
@@ -39,6 +52,7 @@ def build_fastcall(force: bool = False) -> Path:
     include = [INCLUDE, sysconfig.get_paths()["include"], root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
                Path(_nvcc()).resolve().parent.parent / "include"]
     cmd = [cxx, "-O2", "-Wall", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DMOE_RD_BUILT_FOR="{fastcall_stamp()}"',
            *[f"-I{i}" for i in include], str(src), "-o", str(FASTCALL), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
            "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)

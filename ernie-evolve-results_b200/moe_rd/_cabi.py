@@ -88,11 +88,15 @@ FAST_ENTRIES = ("moe_rd_sort_workspace_bytes", "moe_rd_sort_tokens", "moe_rd_uns
 
 
 def _load_fast(L: ctypes.CDLL):
+    from ._build import FASTCALL, fastcall_fits
+    if not FASTCALL.exists():
+        return _NotLoaded()  # the calls still run, from Python
     try:
+        if not fastcall_fits():
+            raise ImportError("it was compiled for another torch or Python")
         from . import _fastcall
-    except ImportError as e:  # the calls still run, from Python
-        if (_LIB_PATH.parent / "_fastcall.so").exists():
-            warnings.warn(f"moe_rd: _fastcall.so does not load with this torch, rebuild it with `python -m moe_rd._build --force`: {e}")
+    except ImportError as e:
+        warnings.warn(f"moe_rd: _fastcall.so does not load with this torch, rebuild it with `python -m moe_rd._build --force`: {e}")
         return _NotLoaded()
     _fastcall.bind(*(ctypes.cast(getattr(L, name), ctypes.c_void_p).value for name in FAST_ENTRIES))
     return _fastcall

@@ -204,3 +204,28 @@ def test_tangents_of_forward_mode_are_refused():
                 call()
             with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+def test_a_module_of_another_torch_is_not_loaded_and_is_built_anew(monkeypatch, tmp_path):
+    import shutil
+    import subprocess
+    from moe_rd import _build
+    L = _cabi.lib()
+    assert _cabi._load_fast(L) is _cabi.fast                         # compiled for this one
+    monkeypatch.setattr(torch, "__version__", "1.0.0+other")
+    with pytest.warns(UserWarning, match="rebuild"):
+        assert isinstance(_cabi._load_fast(L), _cabi._NotLoaded)
+    there = tmp_path / "_fastcall.so"
+    shutil.copy2(_build.FASTCALL, there)
+    monkeypatch.setattr(_build, "FASTCALL", there)
+    built = []
+
+    def run(cmd, **kw):
+        built.append(cmd)
+        raise InterruptedError
+    monkeypatch.setattr(subprocess, "run", run)
+    with pytest.raises(InterruptedError):
+        _build.build_fastcall()
+    assert any("1.0.0+other" in a for a in built[0])
+    monkeypatch.undo()
+    assert _build.build_fastcall() == _build.FASTCALL
