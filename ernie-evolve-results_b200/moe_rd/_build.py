@@ -4,6 +4,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -40,7 +41,8 @@ def fastcall_fits() -> bool:
 
 
 def build_fastcall(force: bool = False) -> Path:
-    """csrc/fastcall.cpp against the headers of the installed torch and Python."""
+    """csrc/fastcall.cpp against the headers of the installed torch and Python.  Written beside the module and moved in its
+    place; a module that is out of date does not stay where the new one fails."""
     src = CSRC / "fastcall.cpp"
     if (not force and FASTCALL.exists() and all(FASTCALL.stat().st_mtime >= d.stat().st_mtime for d in (src, INCLUDE / "moe_rd.h"))
             and fastcall_fits()):
@@ -48,16 +50,20 @@ def build_fastcall(force: bool = False) -> Path:
     import sysconfig
     import torch
     root = Path(torch.__file__).resolve().parent
+    FASTCALL.unlink(missing_ok=True)
+    made = FASTCALL.with_name(f"{FASTCALL.name}.{os.getpid()}.tmp")
     cxx = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else "g++"
     include = [INCLUDE, sysconfig.get_paths()["include"], root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
                Path(_nvcc()).resolve().parent.parent / "include"]
     cmd = [cxx, "-O2", "-Wall", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            f'-DMOE_RD_BUILT_FOR="{fastcall_stamp()}"',
-           *[f"-I{i}" for i in include], str(src), "-o", str(FASTCALL), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           *[f"-I{i}" for i in include], str(src), "-o", str(made), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
            "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
+        made.unlink(missing_ok=True)
         raise RuntimeError(f"g++ failed on {src.name}:\n{r.stdout}\n{r.stderr}")
+    os.replace(made, FASTCALL)
     return FASTCALL
 
 
@@ -65,7 +71,10 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     with ThreadPoolExecutor(max_workers=1) as ex:  # beside nvcc
         fastcall = ex.submit(build_fastcall, force)
         lib = build_library(force, verbose)
-        fastcall.result()
+        try:
+            fastcall.result()
+        except Exception as e:  # no torch headers, no g++: the library is whole and every call runs without the module
+            warnings.warn(f"moe_rd: _fastcall.so is not built, the calls go through Python: {e}")
     return lib
 
 

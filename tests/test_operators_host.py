@@ -229,3 +229,24 @@ def test_a_module_of_another_torch_is_not_loaded_and_is_built_anew(monkeypatch, 
     assert any("1.0.0+other" in a for a in built[0])
     monkeypatch.undo()
     assert _build.build_fastcall() == _build.FASTCALL
+
+
+@pytest.mark.parametrize("why", ["compiler", "headers"])
+def test_the_library_is_built_where_the_module_cannot_be(monkeypatch, tmp_path, why):
+    import subprocess
+    from moe_rd import _build
+    monkeypatch.setattr(_build, "FASTCALL", tmp_path / "_fastcall.so")
+    (tmp_path / "_fastcall.so").write_bytes(b"of other sources")
+    run = subprocess.run
+
+    def without(cmd, **kw):
+        if "nvcc" in cmd[0]:
+            return run(cmd, **kw)
+        if why == "compiler":
+            raise FileNotFoundError("g++")
+        return subprocess.CompletedProcess(cmd, 1, "", "torch/csrc/autograd/python_variable.h: No such file")
+    monkeypatch.setattr(subprocess, "run", without)
+    with pytest.warns(UserWarning, match="_fastcall.so is not built"):
+        assert _build.build() == _build.LIB and _build.LIB.exists()
+    assert list(tmp_path.iterdir()) == []
+    assert isinstance(_cabi._load_fast(_cabi.lib()), _cabi._NotLoaded)
