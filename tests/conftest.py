@@ -1,4 +1,5 @@
 import sys
+import zlib
 from pathlib import Path
 
 import pytest
@@ -25,3 +26,10 @@ def pytest_collection_modifyitems(config, items):
     for item in items:
         if "gpu" in item.keywords:
             item.add_marker(skip)
+
+
+@pytest.fixture(autouse=True)
+def _draws_of_its_own(request):
+    """What a test draws from torch's global generator depends on its name alone, so that a failure comes again."""
+    import torch
+    torch.manual_seed(zlib.crc32(request.node.nodeid.encode()))
