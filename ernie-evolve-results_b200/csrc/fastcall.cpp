@@ -6,7 +6,7 @@
 //   False          anything else: the Python function that called goes its own way, which knows every other case and the
 //                  reason of every refusal.  A C entry that reports an error comes out here too (its outputs are then
 //                  written again, or refused with their reason).
-// A call with `out` costs the host 2.3 to 2.9 us this way and 8.3 to 10.7 the Python way; the launch is 2.3 of both.  The
+// A call with `out` costs the host 2.4 to 3.2 us this way and 8.6 to 11.7 the Python way; the launch is 2.3 of both.  The
 // smallest calls take the GPU 3 to 6 us, so that a decode step pays for the host in every one of them.
 //
 // The C entries come as addresses from the Python side, which has loaded the library (bind).

@@ -100,8 +100,8 @@ __device__ __forceinline__ void clear_own_rows(const UnsortGradArgs& a, unsigned
 }
 
 // KT slots at a time; NEED_W: grad_weights is wanted (and y is read).  The compiler left alone takes 128 registers for
-// KT = 8, two blocks per SM; with 80 and three blocks 32768 tokens x 2048, K = 8 take 364 us instead of 401, and with four
-// warps a token instead of eight 346 us (6.2 TB/s).  KT = 2 is fastest left alone (108 us against 123 for 16384 x 4096).
+// KT = 8, two blocks per SM; with 80 and three blocks 32768 tokens x 2048, K = 8 take 366 us (6.2 TB/s) instead of 381, and
+// with eight warps a token instead of four 385.  KT = 2 is fastest left alone (110 us against 123 for 16384 x 4096).
 template <int DT, int KT, bool NEED_W>
 __global__ void __launch_bounds__(kGradThreads, KT == 8 ? 3 : KT == 4 ? 4 : 0) unsort_grad_kernel(const UnsortGradArgs a) {
   constexpr int NE = RowVec<DT>::N;
